@@ -21,6 +21,8 @@ KERNEL_NAMES = {0: "macro-tile", 1: "matrix-vector", 2: "streaming, few rows", 3
                 4: "short K, tiles walked by resident workgroups",
                 5: "256 x 128 tiles walked by one resident workgroup per CU"}
 
+F32, F16, BF16 = range(3)   # element types of the 4-bit linear layer and of orthogonalize
+
 OK, ERR_ARG, ERR_NO_DEVICE, ERR_HIP, ERR_ALLOC, ERR_RANGE, ERR_ARCH = range(7)
 
 BLK_FIELDS = [
@@ -119,6 +121,14 @@ SIGNATURES = {
     "cake_hip_linear_forward_wt": (_i, [_fp, _fp, _fp, _fp, _i, _i, _i, C.c_void_p, _dp]),
     "cake_hip_sgemm_nt": (_i, [_fp, _fp, _fp, _i, _i, _i, _i, C.POINTER(_i), C.c_void_p, _dp]),
     "cake_hip_linear_backward": (_i, [_fp] * 6 + [_i, _i, _i, C.c_void_p, _dp]),
+    "cake_hip_q4_size": (C.c_size_t, [_i] * 5),
+    "cake_hip_q4_pack": (_i, [_fp] * 4 + [_i] * 4 + [C.c_void_p, _dp]),
+    "cake_hip_q4_quantize": (_i, [_fp, _i, _fp] + [_i] * 5 + [C.c_void_p, _dp]),
+    "cake_hip_q4_dequantize": (_i, [_fp, _fp] + [_i] * 6 + [C.c_void_p, _dp]),
+    "cake_hip_linear_q4_workspace": (C.c_size_t, [_i] * 4),
+    "cake_hip_linear_q4_forward": (_i, [_fp] * 4 + [_i] * 7 + [C.c_void_p, C.c_void_p, _dp]),
+    "cake_hip_orthogonalize_workspace": (C.c_size_t, [_i] * 3),
+    "cake_hip_orthogonalize": (_i, [_fp, _fp] + [_i] * 5 + [C.c_double] * 4 + [C.c_void_p, C.c_void_p, _dp]),
     "cake_hip_autotune": (_i, [_i, _i, _i, C.c_double, C.POINTER(Plan), _dp, _dp]),
     "cake_hip_tune_save": (_i, [C.c_char_p]),
     "cake_hip_tune_load": (_i, [C.c_char_p, C.POINTER(_i)]),

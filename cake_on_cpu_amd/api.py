@@ -16,7 +16,7 @@ import subprocess
 import numpy as np
 
 from . import _lib
-from ._lib import KMN, MKN, NKM, NA, BlkDims, CpuCntx, DeviceInfo, Plan, check, load
+from ._lib import KMN, MKN, NKM, NA, BlkDims, CakeHipError, CpuCntx, DeviceInfo, Plan, check, load
 
 
 # ----------------------------------------------------------------------------
@@ -497,6 +497,166 @@ def linear_backward(grad_y, x, w, grad_x, grad_w, grad_bias, M, N, K, timed=True
                                           _opt_ptr(grad_x, "grad_x"), _opt_ptr(grad_w, "grad_w"),
                                           _opt_ptr(grad_bias, "grad_bias"), M, N, K,
                                           _stream(grad_y, x, w), C.byref(secs) if timed else None), "linear_backward")
+    return secs.value
+
+
+# ----------------------------------------------------------------------------
+# the linear layer with 4-bit weights, orthogonalised updates
+# ----------------------------------------------------------------------------
+_TYPE_CODES = {"float32": _lib.F32, "float16": _lib.F16, "bfloat16": _lib.BF16}
+
+
+def element_type(dtype) -> int:
+    """CAKE_HIP_F32 / F16 / BF16 of a torch or numpy dtype or its name."""
+    name = dtype if isinstance(dtype, str) else str(dtype).replace("torch.", "") if not isinstance(dtype, type) else np.dtype(dtype).name
+    if name not in _TYPE_CODES:
+        raise TypeError(f"element type {dtype}: float32, float16 or bfloat16 needed")
+    return _TYPE_CODES[name]
+
+
+def _any_ptr(a, what: str, of: int | None = None) -> int:
+    """Address of a contiguous array of any element type (uint8, or `of` = an element type's code)."""
+    if _is_torch(a):
+        ok = a.is_contiguous()
+        where = a.data_ptr()
+    elif isinstance(a, np.ndarray):
+        ok = a.flags["C_CONTIGUOUS"]
+        where = a.ctypes.data
+    else:
+        raise TypeError(f"{what} must be a numpy array or torch tensor")
+    if not ok:
+        raise TypeError(f"{what} must be contiguous")
+    if of is None:
+        if str(a.dtype).replace("torch.", "") != "uint8":
+            raise TypeError(f"{what} must be uint8, got {a.dtype}")
+    elif element_type(a.dtype) != of:
+        raise TypeError(f"{what} is {a.dtype}, another element type than its companions")
+    return where
+
+
+class Q4Weight:
+    """A weight matrix v[N][K] in 4 bits, v = (code - zero) * scale per run of `group` columns: the packed
+    bytes (numpy or torch uint8, in the library's own order) and what they hold.  It is made by q4_pack
+    or q4_quantize; q4_of wraps bytes that were stored."""
+    __slots__ = ("data", "N", "K", "group", "scale_type", "with_zeros")
+
+    def __init__(self, data, N, K, group, scale_type, with_zeros):
+        self.data, self.N, self.K, self.group = data, N, K, group
+        self.scale_type, self.with_zeros = scale_type, bool(with_zeros)
+
+
+def q4_size(N, K, group=128, scale_dtype="float32", zeros=False) -> int:
+    """Bytes of the packed form."""
+    n = load().cake_hip_q4_size(N, K, group, element_type(scale_dtype), int(zeros))
+    if n == 0 and N > 0 and K > 0:
+        raise CakeHipError(_lib.ERR_ARG, "q4_size", load().cake_hip_last_error().decode())
+    return n
+
+
+def _bytes_like(ref, n):
+    if _is_torch(ref):
+        import torch
+        return torch.empty(n, dtype=torch.uint8, device=ref.device)
+    # a little more than needed, so that the packed bytes can start on 16
+    raw = np.empty(n + 16, np.uint8)
+    skip = -raw.ctypes.data % 16
+    return raw[skip:skip + n]
+
+
+def q4_of(data, N, K, group, scale_dtype, zeros) -> Q4Weight:
+    """Packed bytes that an earlier q4_pack or q4_quantize made, with what they were made for."""
+    _any_ptr(data, "packed weights")
+    _need(data, q4_size(N, K, group, scale_dtype, zeros), "packed weights")
+    return Q4Weight(data, N, K, group, element_type(scale_dtype), zeros)
+
+
+def q4_pack(codes, scales, zeros, N, K, group=128, timed=False) -> Q4Weight:
+    """codes[N][(K + 1) // 2] (uint8, even columns in the low half of a byte), scales and zeros
+    [N][ceil(K / group)] of one element type (zeros None: 8 everywhere) as packed weights."""
+    st = element_type(scales.dtype)
+    q = Q4Weight(_bytes_like(codes, q4_size(N, K, group, scales.dtype, zeros is not None)), N, K, group, st, zeros is not None)
+    runs = N * -(-K // group)
+    _need(codes, N * ((K + 1) // 2), "codes")
+    _need(scales, runs, "scales")
+    if zeros is not None:
+        _need(zeros, runs, "zeros")
+    secs = C.c_double(0.0)
+    check(load().cake_hip_q4_pack(_any_ptr(codes, "codes"), _any_ptr(scales, "scales", st),
+                                  None if zeros is None else _any_ptr(zeros, "zeros", st), _any_ptr(q.data, "q"), N, K, group, st,
+                                  _stream(codes, scales), C.byref(secs) if timed else None), "q4_pack")
+    return q
+
+
+def q4_quantize(w, N, K, group=128, zeros=False, scale_dtype="float32", timed=False) -> Q4Weight:
+    """w[N][K] in 4 bits: scales max|w| / 7 around code 8, or with `zeros` the range's / 15 and a zero point
+    (the full definition is in include/cake_hip.h)."""
+    _need(w, N * K, "w")
+    st, wt = element_type(scale_dtype), element_type(w.dtype)
+    q = Q4Weight(_bytes_like(w, q4_size(N, K, group, scale_dtype, zeros)), N, K, group, st, zeros)
+    secs = C.c_double(0.0)
+    check(load().cake_hip_q4_quantize(_any_ptr(w, "w", wt), wt, _any_ptr(q.data, "q"), N, K, group, st, int(q.with_zeros),
+                                      _stream(w), C.byref(secs) if timed else None), "q4_quantize")
+    return q
+
+
+def q4_dequantize(q: Q4Weight, w, timed=False) -> float:
+    """The values that packed weights stand for, into w[N][K] of any element type.  Returns seconds (0 with timed=False)."""
+    _need(w, q.N * q.K, "w")
+    wt = element_type(w.dtype)
+    secs = C.c_double(0.0)
+    check(load().cake_hip_q4_dequantize(_any_ptr(q.data, "q"), _any_ptr(w, "w", wt), wt, q.N, q.K, q.group, q.scale_type,
+                                        int(q.with_zeros), _stream(w, q.data), C.byref(secs) if timed else None), "q4_dequantize")
+    return secs.value
+
+
+def linear_q4_workspace(M, N, K, dtype="float32") -> int:
+    """Bytes of device memory linear_q4_forward wants for M rows of x (0 for a few)."""
+    return load().cake_hip_linear_q4_workspace(M, N, K, element_type(dtype))
+
+
+def linear_q4_forward(x, q: Q4Weight, bias, y, M, workspace=None, timed=True) -> float:
+    """y[M][N] = x[M][K] . v[N][K]^T + bias[N] (bias may be None); x, bias and y of one element type.
+    workspace: a uint8 device tensor of linear_q4_workspace bytes, or None for the library's own.
+    Returns seconds (0 with timed=False, which makes the call asynchronous on device operands)."""
+    t = element_type(x.dtype)
+    N, K = q.N, q.K
+    _need(x, M * K, "x")
+    _need(y, M * N, "y")
+    if bias is not None:
+        _need(bias, N, "bias")
+    if workspace is not None:
+        _need(workspace, load().cake_hip_linear_q4_workspace(M, N, K, t), "workspace")
+    secs = C.c_double(0.0)
+    check(load().cake_hip_linear_q4_forward(_any_ptr(x, "x", t), _any_ptr(q.data, "q"),
+                                            None if bias is None else _any_ptr(bias, "bias", t), _any_ptr(y, "y", t), t, M, N, K,
+                                            q.group, q.scale_type, int(q.with_zeros),
+                                            None if workspace is None else _any_ptr(workspace, "workspace"),
+                                            _stream(x, q.data, y), C.byref(secs) if timed else None), "linear_q4_forward")
+    return secs.value
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize_workspace(batch, rows, cols) -> int:
+    """Bytes of device memory orthogonalize wants."""
+    return load().cake_hip_orthogonalize_workspace(batch, rows, cols)
+
+
+def orthogonalize(g, out, batch, rows, cols, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, workspace=None, timed=True) -> float:
+    """Newton-Schulz iterations on g[batch][rows][cols] into out (of g's element type; may be g):
+    x = g / (|g| + eps), then `steps` times a = x x^T, x = c0 x + (c1 a + c2 a a) x.
+    Returns seconds (0 with timed=False)."""
+    t = element_type(g.dtype)
+    _need(g, batch * rows * cols, "g")
+    _need(out, batch * rows * cols, "out")
+    if workspace is not None:
+        _need(workspace, load().cake_hip_orthogonalize_workspace(batch, rows, cols), "workspace")
+    c0, c1, c2 = coefficients
+    secs = C.c_double(0.0)
+    check(load().cake_hip_orthogonalize(_any_ptr(g, "g", t), _any_ptr(out, "out", t), t, batch, rows, cols, steps, c0, c1, c2, eps,
+                                        None if workspace is None else _any_ptr(workspace, "workspace"),
+                                        _stream(g, out), C.byref(secs) if timed else None), "orthogonalize")
     return secs.value
 
 

@@ -2,6 +2,7 @@
 // host/device operand staging, workspace ownership, timing, kernel dispatch.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -16,6 +17,7 @@
 #include "blockdims.hpp"
 #include "cake_hip.h"
 #include "kernels.hpp"
+#include "low_bits.hpp"
 #include "planner.hpp"
 
 namespace {
@@ -120,7 +122,7 @@ struct Context {
     cake_hip_device_t info{};
     DeviceModel model;
     DeviceBuffer stage[STAGE_SLOTS];  // device copies of host operands
-    DeviceBuffer splitk, gemv, conv, conv_taps, conv_filters, tables, unpacked, linear, turned;
+    DeviceBuffer splitk, gemv, conv, conv_taps, conv_filters, tables, unpacked, linear, turned, linear_q4, orthogonal;
     hipStream_t own_stream = nullptr;   // what a NULL stream argument means on this context (default context: the null stream)
     hipEvent_t ev[2] = {nullptr, nullptr};
     hipEvent_t fam[2] = {nullptr, nullptr};
@@ -136,7 +138,8 @@ struct Context {
     bool noalloc_call = false;
     size_t noalloc_used = 0;
 
-    DeviceBuffer* compute_buffers[9] = {&splitk, &gemv, &conv, &conv_taps, &conv_filters, &tables, &unpacked, &linear, &turned};
+    DeviceBuffer* compute_buffers[11] = {&splitk, &gemv, &conv, &conv_taps, &conv_filters, &tables, &unpacked, &linear, &turned,
+                                         &linear_q4, &orthogonal};
     int create_events()
     {
         for (hipEvent_t* e : {&ev[0], &ev[1], &fam[0], &fam[1]})
@@ -2111,6 +2114,296 @@ int cake_hip_linear_backward(const float* grad_y, const float* x, const float* w
     if (grad_w && (st = stage_out(gwo, stream))) return st;
     if (grad_bias && (st = stage_out(gbo, stream))) return st;
     return CAKE_HIP_OK;
+}
+
+// ---- 4-bit weights, orthogonalised updates ---------------------------------------------
+
+// The calling thread's device, put back at the end of a call that runs on the context's.
+struct DeviceGuard {
+    int before = -1;
+    int enter()
+    {
+        int now = 0;
+        HIP_TRY(hipGetDevice(&now));
+        if (now == cur().device) return CAKE_HIP_OK;
+        HIP_TRY(hipSetDevice(cur().device));
+        before = now;
+        return CAKE_HIP_OK;
+    }
+    ~DeviceGuard()
+    {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// stage_in for operands of any type that also refuses memory of another device.
+static int any_in(const void* p, size_t bytes, int slot, bool copy, Operand* op, const char* what)
+{
+    hipPointerAttribute_t attr;
+    if (bytes && hipPointerGetAttributes(&attr, p) == hipSuccess) {
+        if (attr.type == hipMemoryTypeDevice && attr.device != cur().device)
+            return fail(CAKE_HIP_ERR_ARG, "%s is memory of device %d, the context's device is %d", what, attr.device, cur().device);
+        if (attr.type == hipMemoryTypeDevice || attr.type == hipMemoryTypeManaged) {
+            op->dev = static_cast<float*>(const_cast<void*>(p));
+            op->bytes = bytes;
+            return CAKE_HIP_OK;
+        }
+    } else {
+        (void)hipGetLastError();   // plain host memory is reported as an error
+    }
+    return stage_in(static_cast<const float*>(p), bytes, slot, copy, op);
+}
+
+// A caller's workspace, or `buf` grown to the size.
+static int workspace_of(void* given, size_t bytes, size_t align, DeviceBuffer& buf, void** out)
+{
+    if (!given) {
+        if (bytes) {
+            int st = buf.reserve(bytes);
+            if (st) return st;
+        }
+        *out = buf.ptr;
+        return CAKE_HIP_OK;
+    }
+    if ((uintptr_t)given % align) return fail(CAKE_HIP_ERR_ARG, "workspace is not %zu-byte aligned", align);
+    if (bytes) {
+        hipPointerAttribute_t attr;
+        if (hipPointerGetAttributes(&attr, given) != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != cur().device) {
+            (void)hipGetLastError();
+            return fail(CAKE_HIP_ERR_ARG, "workspace must be memory of device %d", cur().device);
+        }
+    }
+    *out = given;
+    return CAKE_HIP_OK;
+}
+
+static bool element_type_ok(int type) { return type == CAKE_HIP_F32 || type == CAKE_HIP_F16 || type == CAKE_HIP_BF16; }
+
+static int q4_args_ok(int N, int K, int group, int scale_type)
+{
+    if (N < 0 || K < 0) return fail(CAKE_HIP_ERR_ARG, "negative dimension");
+    if (group != 32 && group != 64 && group != 128) return fail(CAKE_HIP_ERR_ARG, "group of %d weights (32, 64 or 128)", group);
+    if (!element_type_ok(scale_type)) return fail(CAKE_HIP_ERR_ARG, "unknown scale type %d", scale_type);
+    // rows and columns are padded to whole tiles in 32-bit arithmetic
+    if (!fits_int((double)N * K) || N > 0x7FFFFF00 || K > 0x7FFFFF00)
+        return fail(CAKE_HIP_ERR_RANGE, "weights of %dx%d exceed 2^31 elements", N, K);
+    return CAKE_HIP_OK;
+}
+
+static int q4_aligned(const Operand& q)
+{
+    return (uintptr_t)q.dev % 16 ? fail(CAKE_HIP_ERR_ARG, "packed weights are not 16-byte aligned") : (int)CAKE_HIP_OK;
+}
+
+size_t cake_hip_q4_size(int N, int K, int group, int scale_type, int with_zeros)
+{
+    if (q4_args_ok(N, K, group, scale_type)) return 0;
+    return q4_layout(N, K, group, scale_type, with_zeros != 0).bytes;
+}
+
+int cake_hip_q4_pack(const unsigned char* codes, const void* scales, const void* zeros, void* q, int N, int K, int group,
+                     int scale_type, void* stream_, double* seconds)
+{
+    if (seconds) *seconds = 0;
+    int st = q4_args_ok(N, K, group, scale_type);
+    if (st) return st;
+    if (N == 0 || K == 0) return CAKE_HIP_OK;
+    if (!codes || !scales || !q) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
+    if ((st = ensure_init())) return st;
+    std::lock_guard<std::recursive_mutex> lock(cur().mutex);
+    DeviceGuard guard;
+    if ((st = guard.enter())) return st;
+    hipStream_t stream = pick_stream(stream_);
+    const Q4Layout lay = q4_layout(N, K, group, scale_type, zeros != nullptr);
+    const size_t scale_bytes = (size_t)N * ((K + group - 1) / group) * type_bytes(scale_type);
+    Operand co, so, zo, qo;
+    if ((st = any_in(codes, (size_t)N * (((size_t)K + 1) / 2), 0, true, &co, "codes"))) return st;
+    if ((st = any_in(scales, scale_bytes, 1, true, &so, "scales"))) return st;
+    if (zeros && (st = any_in(zeros, scale_bytes, 2, true, &zo, "zeros"))) return st;
+    if ((st = any_in(q, lay.bytes, 3, false, &qo, "packed weights"))) return st;
+    if ((st = q4_aligned(qo))) return st;
+    Timer timer(stream, seconds);
+    if ((st = timer.start())) return st;
+    st = timer.family(4, [&] {
+        return launch_q4_pack(reinterpret_cast<const unsigned char*>(co.dev), so.dev, zeros ? zo.dev : nullptr, qo.dev, lay, stream);
+    });
+    if (st) return st;
+    if ((st = timer.stop())) return st;
+    return stage_out(qo, stream);
+}
+
+// quantize and dequantize: one matrix, one packed form, either way
+static int q4_convert(const void* src, void* dst, bool to_codes, int w_type, int N, int K, int group, int scale_type,
+                      int with_zeros, void* stream_, double* seconds)
+{
+    if (seconds) *seconds = 0;
+    int st = q4_args_ok(N, K, group, scale_type);
+    if (st) return st;
+    if (!element_type_ok(w_type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", w_type);
+    if (N == 0 || K == 0) return CAKE_HIP_OK;
+    if (!src || !dst) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
+    if ((st = ensure_init())) return st;
+    std::lock_guard<std::recursive_mutex> lock(cur().mutex);
+    DeviceGuard guard;
+    if ((st = guard.enter())) return st;
+    hipStream_t stream = pick_stream(stream_);
+    const Q4Layout lay = q4_layout(N, K, group, scale_type, with_zeros != 0);
+    const size_t w_bytes = (size_t)N * K * type_bytes(w_type);
+    Operand in, out;
+    if ((st = any_in(src, to_codes ? w_bytes : lay.bytes, 0, true, &in, to_codes ? "w" : "packed weights"))) return st;
+    if ((st = any_in(dst, to_codes ? lay.bytes : w_bytes, 1, false, &out, to_codes ? "packed weights" : "w"))) return st;
+    if ((st = q4_aligned(to_codes ? out : in))) return st;
+    Timer timer(stream, seconds);
+    if ((st = timer.start())) return st;
+    st = timer.family(4, [&] {
+        return to_codes ? launch_q4_quantize(in.dev, w_type, out.dev, lay, with_zeros != 0, stream)
+                        : launch_q4_dequantize(in.dev, out.dev, w_type, lay, with_zeros != 0, stream);
+    });
+    if (st) return st;
+    if ((st = timer.stop())) return st;
+    return stage_out(out, stream);
+}
+
+int cake_hip_q4_quantize(const void* w, int w_type, void* q, int N, int K, int group, int scale_type, int with_zeros,
+                         void* stream, double* seconds)
+{
+    return q4_convert(w, q, true, w_type, N, K, group, scale_type, with_zeros, stream, seconds);
+}
+
+int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int group, int scale_type, int with_zeros,
+                           void* stream, double* seconds)
+{
+    return q4_convert(q, w, false, w_type, N, K, group, scale_type, with_zeros, stream, seconds);
+}
+
+size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type)
+{
+    if (linear_dims_ok(M, N, K) || !element_type_ok(type)) return 0;
+    return linear_q4_workspace(M, N, K, type);
+}
+
+int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, void* y, int type, int M, int N, int K,
+                               int group, int scale_type, int with_zeros, void* workspace, void* stream_, double* seconds)
+{
+    if (seconds) *seconds = 0;
+    int st = linear_dims_ok(M, N, K);
+    if (st) return st;
+    if ((st = q4_args_ok(N, K, group, scale_type))) return st;
+    if (!element_type_ok(type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", type);
+    if (M == 0 || N == 0) return CAKE_HIP_OK;
+    if (!y || (K > 0 && (!x || !q))) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
+    if ((st = ensure_init())) return st;
+    std::lock_guard<std::recursive_mutex> lock(cur().mutex);
+    DeviceGuard guard;
+    if ((st = guard.enter())) return st;
+    hipStream_t stream = pick_stream(stream_);
+    const Q4Layout lay = q4_layout(N, K, group, scale_type, with_zeros != 0);
+    const size_t b = type_bytes(type);
+    Operand xo, qo, bo, yo;
+    if ((st = any_in(x, (size_t)M * K * b, 0, true, &xo, "x"))) return st;
+    if ((st = any_in(q, lay.bytes, 1, true, &qo, "packed weights"))) return st;
+    if ((st = q4_aligned(qo))) return st;
+    if (bias && (st = any_in(bias, (size_t)N * b, 2, true, &bo, "bias"))) return st;
+    if ((st = any_in(y, (size_t)M * N * b, 3, false, &yo, "y"))) return st;
+    void* ws = nullptr;
+    if ((st = workspace_of(workspace, linear_q4_workspace(M, N, K, type), 16, cur().linear_q4, &ws))) return st;
+    Timer timer(stream, seconds);
+    if ((st = timer.start())) return st;
+    st = timer.family(M <= 64 ? 2 : 0, [&] {
+        return launch_linear_q4(xo.dev, qo.dev, bias ? bo.dev : nullptr, yo.dev, type, M, lay, with_zeros != 0, ws, cur().model.cus, stream);
+    });
+    if (st) return st;
+    if ((st = timer.stop())) return st;
+    return stage_out(yo, stream);
+}
+
+// How far a singular value from [0, 1] and the polynomial that multiplies it can get in `steps`
+// iterations, and from that the powers of two under which x, a = x x^T and b = c0 + c1 a + c2 a a stay
+// below fp16's 65504 (no entry of a matrix exceeds its largest singular value).
+static int orthogonalize_scales(int steps, double c0, double c1, double c2, OrthogonalizeScales* out)
+{
+    double u = 1.001, widest = u, highest = 0;
+    for (int i = 0; i < steps; ++i) {
+        const double end = u * u;
+        auto poly = [&](double s) { return fabs(c0 + s * (c1 + s * c2)); };
+        double b = fmax(poly(0), poly(end));
+        if (c2 != 0) {   // the polynomial's own vertex
+            const double v = -c1 / (2 * c2);
+            if (v > 0 && v < end) b = fmax(b, poly(v));
+        }
+        highest = fmax(highest, b);
+        double next = u * poly(end);
+        // extremes of sigma poly(sigma^2): c0 + 3 c1 s + 5 c2 s^2 = 0
+        double root[2];
+        int roots = 0;
+        if (c2 != 0) {
+            const double d = 9 * c1 * c1 - 20 * c0 * c2;
+            if (d >= 0) {
+                root[roots++] = (-3 * c1 + sqrt(d)) / (10 * c2);
+                root[roots++] = (-3 * c1 - sqrt(d)) / (10 * c2);
+            }
+        } else if (c1 != 0) {
+            root[roots++] = -c0 / (3 * c1);
+        }
+        for (int r = 0; r < roots; ++r)
+            if (root[r] > 0 && root[r] < end) next = fmax(next, sqrt(root[r]) * poly(root[r]));
+        u = next * 1.001;   // rounding on the way
+        if (!(u <= 1000)) return fail(CAKE_HIP_ERR_ARG, "coefficients %g, %g, %g take a singular value beyond 1000 in step %d", c0, c1, c2, i + 1);
+        widest = fmax(widest, u);
+    }
+    auto power = [](double most) { return most < 3.5 ? 14 : (int)floor(log2(60000.0 / most)); };
+    out->ex = power(widest);
+    out->ea = power(widest * widest);
+    out->eb = power(highest);
+    return CAKE_HIP_OK;
+}
+
+static int orthogonalize_dims_ok(int batch, int rows, int cols)
+{
+    if (batch < 0 || rows < 0 || cols < 0) return fail(CAKE_HIP_ERR_ARG, "negative dimension");
+    if (!fits_int((double)rows * cols)) return fail(CAKE_HIP_ERR_RANGE, "matrix of %dx%d exceeds 2^31 elements", rows, cols);
+    if (batch > 65535) return fail(CAKE_HIP_ERR_RANGE, "batch of %d matrices (65535 at most)", batch);
+    return CAKE_HIP_OK;
+}
+
+size_t cake_hip_orthogonalize_workspace(int batch, int rows, int cols)
+{
+    if (orthogonalize_dims_ok(batch, rows, cols) || batch == 0 || rows == 0 || cols == 0) return 0;
+    return orthogonalize_layout(batch, rows, cols).bytes;
+}
+
+int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1,
+                           double c2, double eps, void* workspace, void* stream_, double* seconds)
+{
+    if (seconds) *seconds = 0;
+    int st = orthogonalize_dims_ok(batch, rows, cols);
+    if (st) return st;
+    if (!element_type_ok(type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", type);
+    if (steps < 1) return fail(CAKE_HIP_ERR_ARG, "%d steps", steps);
+    if (!(eps >= 0) || std::isinf(eps)) return fail(CAKE_HIP_ERR_ARG, "eps %g", eps);
+    OrthogonalizeScales scales;
+    if ((st = orthogonalize_scales(steps, c0, c1, c2, &scales))) return st;
+    if (batch == 0 || rows == 0 || cols == 0) return CAKE_HIP_OK;
+    if (!g || !out) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
+    if ((st = ensure_init())) return st;
+    std::lock_guard<std::recursive_mutex> lock(cur().mutex);
+    DeviceGuard guard;
+    if ((st = guard.enter())) return st;
+    hipStream_t stream = pick_stream(stream_);
+    const size_t bytes = (size_t)batch * rows * cols * type_bytes(type);
+    Operand in, res;
+    if ((st = any_in(g, bytes, 0, true, &in, "g"))) return st;
+    if ((st = any_in(out, bytes, 1, false, &res, "out"))) return st;
+    void* ws = nullptr;
+    if ((st = workspace_of(workspace, orthogonalize_layout(batch, rows, cols).bytes, 256, cur().orthogonal, &ws))) return st;
+    Timer timer(stream, seconds);
+    if ((st = timer.start())) return st;
+    st = timer.family(0, [&] {
+        return launch_orthogonalize(in.dev, res.dev, type, batch, rows, cols, steps, c0, c1, c2, eps, scales, ws, stream);
+    });
+    if (st) return st;
+    if ((st = timer.stop())) return st;
+    return stage_out(res, stream);
 }
 
 // ---- autotuner -----------------------------------------------------------------------

@@ -9,6 +9,7 @@
 #include <cstdint>
 
 #include "blockdims.hpp"
+#include "q4_layout.hpp"
 
 namespace cake {
 
@@ -276,5 +277,29 @@ hipError_t launch_pack(const float* src, float* dst_packed, int rows, int cols, 
 // dst[r*ld + c] = src_packed[offset(r,c)] over the real extent
 hipError_t launch_unpack(const float* src_packed, float* dst, int rows, int cols, int ld,
                          IndexTables tab, int fast, bool rows_fast, hipStream_t stream);
+
+// 4-bit weights (q4_kernels.hip, q4_linear.hip); q is 16-byte aligned, the other operands as their elements
+hipError_t launch_q4_quantize(const void* w, int w_type, void* q, const Q4Layout& lay, bool with_zeros, hipStream_t stream);
+hipError_t launch_q4_dequantize(const void* q, void* w, int w_type, const Q4Layout& lay, bool with_zeros, hipStream_t stream);
+hipError_t launch_q4_pack(const unsigned char* codes, const void* scales, const void* zeros, void* q, const Q4Layout& lay,
+                          hipStream_t stream);
+hipError_t launch_linear_q4(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
+                            bool with_zeros, void* workspace, int cus, hipStream_t stream);
+size_t linear_q4_workspace(int M, int N, int K, int type);
+
+// Newton-Schulz iterations (orthogonalize.hip).  The layout's offsets are bytes into the workspace.
+struct OrthogonalizeLayout {
+    int m, n;                     // the shorter and the longer side
+    int mb, nb;                   // in blocks of 16, even
+    size_t x_halves, a_halves;    // of one matrix of the batch
+    size_t x, xt0, xt1, a, b, partial, bytes;
+};
+// powers of two that the values of x, a and b are multiplied by where they are kept
+struct OrthogonalizeScales {
+    int ex, ea, eb;
+};
+OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols);
+hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1,
+                                double c2, double eps, const OrthogonalizeScales& sc, void* workspace, hipStream_t stream);
 
 }  // namespace cake

@@ -5,7 +5,10 @@ names -- forward / backward, cake_linear_function, cake_linear.
 Tensors on a ROCm device are used in place through their device pointers on
 torch's current stream; CPU tensors are staged by the library.  torch only
 provides memory, streams and autograd bookkeeping; every product, transpose and
-reduction runs in libcake_hip.so."""
+reduction runs in libcake_hip.so.
+
+Beside it stand the same layer with 4-bit weights for serving (forward_q4, cake_linear_q4) and the
+orthogonalised update of its weight in training (orthogonalize, cake_muon), which the reference lacks."""
 from __future__ import annotations
 
 import torch
@@ -98,3 +101,171 @@ class cake_linear(nn.Module):
 
     def extra_repr(self):
         return f"input_features={self.input_features}, output_features={self.output_features}, bias={self.bias is not None}"
+
+
+# ---- the layer with 4-bit weights -------------------------------------------------------
+
+
+def pack_q4(codes, scales, zeros, in_features, group=128):
+    """Packed weights from an existing checkpoint's tensors: codes[N][(K + 1) // 2] (uint8, even columns in the low
+    half of a byte), scales and zeros (or None: 8) [N][ceil(K / group)]."""
+    if codes.dim() != 2 or codes.size(1) != (in_features + 1) // 2:
+        raise ValueError(f"pack_q4: codes {tuple(codes.shape)} do not hold {in_features} columns")
+    want = (codes.size(0), -(-in_features // group))
+    for t, what in ((scales, "scales"), (zeros, "zeros")):
+        if t is not None and tuple(t.shape) != want:
+            raise ValueError(f"pack_q4: {what} {tuple(t.shape)} are not {want}")
+        if t is not None and t.device != codes.device:
+            raise ValueError(f"pack_q4: {what} on {t.device}, codes on {codes.device}")
+    return api.q4_pack(codes.contiguous(), scales.detach().contiguous(), None if zeros is None else zeros.detach().contiguous(),
+                       codes.size(0), in_features, group)
+
+
+def quantize_q4(weight, group=128, zeros=False, scale_dtype=torch.bfloat16):
+    """A weight matrix in 4 bits with one scale (and, with `zeros`, one zero point) for `group` columns of a row."""
+    if weight.dim() != 2:
+        raise ValueError(f"quantize_q4: weight {tuple(weight.shape)} is no matrix")
+    return api.q4_quantize(weight.detach().contiguous(), *weight.shape, group=group, zeros=zeros, scale_dtype=scale_dtype)
+
+
+def dequantize_q4(q, dtype=torch.float32):
+    """The values that packed weights stand for, as a tensor [N][K]."""
+    w = torch.empty((q.N, q.K), dtype=dtype, device=q.data.device)
+    api.q4_dequantize(q, w)
+    return w
+
+
+def _forward_q4(x, q, bias):
+    M = x.size(0)
+    y = torch.empty((M, q.N), dtype=x.dtype, device=x.device)
+    # a workspace from torch's allocator belongs to this call's stream, and to a graph if one is captured
+    need = api.linear_q4_workspace(M, q.N, q.K, x.dtype) if x.is_cuda and M > 1 else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    api.linear_q4_forward(x, q, bias, y, M, workspace=ws, timed=not x.is_cuda)
+    return y
+
+
+class cake_linear_q4_function(torch.autograd.Function):
+    """Gradients of the layer for its input and bias; the packed weights are constants."""
+
+    @staticmethod
+    def forward(ctx, data, q, bias):
+        ctx.q, ctx.dtype = q, data.dtype
+        return _forward_q4(data.detach().contiguous(), q, None if bias is None else bias.detach().contiguous())
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        q, M = ctx.q, grad_output.size(0)
+        g = grad_output.detach().float().contiguous()
+        gx = torch.empty((M, q.K), dtype=torch.float32, device=g.device) if ctx.needs_input_grad[0] else None
+        gb = torch.empty((q.N,), dtype=torch.float32, device=g.device) if ctx.needs_input_grad[2] else None
+        w = dequantize_q4(q) if gx is not None else None
+        api.linear_backward(g, None, w, gx, None, gb, M, q.N, q.K, timed=not g.is_cuda)
+        return None if gx is None else gx.to(ctx.dtype), None, None if gb is None else gb.to(ctx.dtype)
+
+
+def forward_q4(input, q, bias=None):
+    """output[M][N] = input[M][K] . v[N][K]^T (+ bias) with v in 4 bits (pack_q4, quantize_q4).  input is float32,
+    float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias."""
+    if input.dim() != 2 or input.size(1) != q.K:
+        raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
+    if bias is not None and (tuple(bias.shape) != (q.N,) or bias.dtype != input.dtype):
+        raise ValueError(f"forward_q4: bias {tuple(bias.shape)} of {bias.dtype} does not match {q.N} outputs of {input.dtype}")
+    if input.device != q.data.device or (bias is not None and bias.device != input.device):
+        raise ValueError(f"forward_q4: input on {input.device}, weights on {q.data.device}")
+    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
+        return cake_linear_q4_function.apply(input, q, bias)
+    return _forward_q4(input.contiguous(), q, None if bias is None else bias.contiguous())
+
+
+class cake_linear_q4(nn.Module):
+    """cake_linear with its weight held in 4 bits: cake_linear_q4.of(layer) for a trained layer, or of
+    packed weights.  The packed bytes are a buffer, so .to(device) and state_dict carry them."""
+
+    def __init__(self, q, bias=None):
+        super().__init__()
+        self.input_features, self.output_features = q.K, q.N
+        self.group, self.scale_type, self.with_zeros = q.group, q.scale_type, q.with_zeros
+        self.register_buffer("packed", q.data)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone())
+
+    @classmethod
+    def of(cls, layer, group=128, zeros=False, scale_dtype=torch.bfloat16):
+        """From a layer with .weight and .bias (cake_linear, nn.Linear)."""
+        return cls(quantize_q4(layer.weight, group, zeros, scale_dtype), layer.bias)
+
+    @property
+    def weight_q4(self):
+        return api.Q4Weight(self.packed, self.output_features, self.input_features, self.group, self.scale_type, self.with_zeros)
+
+    def forward(self, data):
+        flat = data.reshape(-1, self.input_features)
+        bias = None if self.bias is None else self.bias.to(data.dtype)
+        return forward_q4(flat, self.weight_q4, bias).reshape(*data.shape[:-1], self.output_features)
+
+    def extra_repr(self):
+        return (f"input_features={self.input_features}, output_features={self.output_features}, bias={self.bias is not None}, "
+                f"group={self.group}, zeros={self.with_zeros}")
+
+
+# ---- the update of a weight matrix in training ---------------------------------------------
+
+
+def orthogonalize(grad, steps=5, coefficients=api.NEWTON_SCHULZ, eps=1e-7):
+    """Newton-Schulz iterations on the last two dimensions (leading ones are a batch): a tensor like `grad` whose
+    matrices have their singular values moved close to 1.  Not differentiable."""
+    if grad.dim() < 2:
+        raise ValueError(f"orthogonalize: {tuple(grad.shape)} is no matrix")
+    rows, cols = grad.shape[-2:]
+    g = grad.detach().contiguous()
+    out = torch.empty_like(g)
+    if g.numel() == 0:
+        return out
+    batch = g.numel() // (rows * cols)
+    ws = torch.empty(api.orthogonalize_workspace(batch, rows, cols), dtype=torch.uint8, device=g.device) if g.is_cuda else None
+    api.orthogonalize(g, out, batch, rows, cols, steps, coefficients, eps, workspace=ws, timed=not g.is_cuda)
+    return out
+
+
+class cake_muon(torch.optim.Optimizer):
+    """Momentum with orthogonalised updates for weight matrices (cake_linear.weight and the like; biases and
+    other vectors belong to another optimiser):
+        b = momentum * b + grad,  u = grad + momentum * b  (b without nesterov)
+        w = w - lr * weight_decay * w - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
+    Matrices of one shape are orthogonalised in one call."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=api.NEWTON_SCHULZ,
+                 eps=1e-7):
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps))
+        for group in self.param_groups:
+            for w in group["params"]:
+                if w.dim() != 2:
+                    raise ValueError(f"cake_muon: parameter {tuple(w.shape)} is no matrix")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            alike = {}
+            for w in group["params"]:
+                if w.grad is None:
+                    continue
+                state = self.state[w]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros_like(w)
+                b = state["momentum"].mul_(group["momentum"]).add_(w.grad)
+                u = w.grad.add(b, alpha=group["momentum"]) if group["nesterov"] else b
+                alike.setdefault((tuple(w.shape), w.dtype, w.device), []).append((w, u))
+            for (shape, _, _), pairs in alike.items():
+                us = torch.stack([u for _, u in pairs]) if len(pairs) > 1 else pairs[0][1].unsqueeze(0)
+                done = orthogonalize(us, group["steps"], group["coefficients"], group["eps"])
+                scale = max(1.0, shape[0] / shape[1]) ** 0.5
+                for i, (w, _) in enumerate(pairs):
+                    if group["weight_decay"]:
+                        w.mul_(1 - group["lr"] * group["weight_decay"])
+                    w.add_(done[i], alpha=-group["lr"] * scale)
+        return loss

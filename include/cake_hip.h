@@ -404,6 +404,74 @@ int cake_hip_linear_backward(const float* grad_y, const float* x, const float* w
                              float* grad_w, float* grad_bias, int M, int N, int K, void* stream,
                              double* seconds);
 
+/* ---- the linear layer with 4-bit weights ---------------------------------- */
+/* Element types of the operators below.  (Everything above is fp32.) */
+enum { CAKE_HIP_F32 = 0, CAKE_HIP_F16 = 1, CAKE_HIP_BF16 = 2 };
+
+/* A weight matrix v[N][K] in 4 bits: code c[n][k] in 0..15 stands for (c - z) * s with one scale s and
+ * one zero point z for each run of `group` columns of a row (group 32, 64 or 128; the last run of a row
+ * may be short).  Scales and zero points are kept in scale_type; with_zeros == 0 keeps no zero points
+ * and stands for z = 8.  The packed form is the library's own: cake_hip_q4_size bytes (0 for
+ * arguments it does not take), 16-byte aligned, codes in the order the matrix pipe takes them, scales and
+ * zero points behind; the same packed weights serve x of every type.  It has no counterpart
+ * in the reference, whose weights are fp32 (src/linear.cpp:12-50).
+ *
+ * These entry points and cake_hip_orthogonalize take host or device operands like all others, except that
+ * memory of another device than the current context's is refused (CAKE_HIP_ERR_ARG), and they
+ * leave the calling thread's current device as it was. */
+size_t cake_hip_q4_size(int N, int K, int group, int scale_type, int with_zeros);
+
+/* Codes of an existing checkpoint into the packed form: codes[N][(K + 1) / 2] with column 2 j of a row in
+ * the low half of its byte j and column 2 j + 1 in the high half, scales and zeros
+ * [N][(K + group - 1) / group] in scale_type; zeros == NULL packs without zero points.  Zero points need
+ * not be whole numbers. */
+int cake_hip_q4_pack(const unsigned char* codes, const void* scales, const void* zeros, void* q, int N, int K,
+                     int group, int scale_type, void* stream, double* seconds);
+
+/* w[N][K] (w_type) into packed codes.  Without zero points s = max|w| / 7 and
+ * c = clamp(round(w / s), -8, 7) + 8; with them lo = min(w, 0), hi = max(w, 0), s = (hi - lo) / 15,
+ * z = clamp(round(-lo / s), 0, 15), c = clamp(round(w / s) + z, 0, 15).  s is rounded to fp32 and then to
+ * scale_type before anything is divided by it; the quotients are rounded as real numbers, ties to
+ * even, whatever scale_type is.  A run of zeros (or one whose scale rounds to 0) gets s = 0, c = z = 8.  Weights
+ * have to be finite: a run that holds a NaN or an infinity comes back as NaN or infinities, and so does one
+ * whose scale overflows fp16. */
+int cake_hip_q4_quantize(const void* w, int w_type, void* q, int N, int K, int group, int scale_type, int with_zeros,
+                         void* stream, double* seconds);
+
+/* w[n][k] = (c - z) * s, rounded to fp32 and then to w_type. */
+int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int group, int scale_type, int with_zeros,
+                           void* stream, double* seconds);
+
+/* y[M][N] = x[M][K] . v[N][K]^T (+ bias[N] on every row when bias != NULL); x, bias and y are of `type`.
+ * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and zero points are applied to a
+ * run's sum in fp32, and y is rounded once.  The order of the sums depends on the sizes alone.  An infinity in x
+ * may come out as NaN in that row of y.  workspace: device memory of cake_hip_linear_q4_workspace bytes
+ * (0 for a few rows of x), 16-byte aligned, or NULL for a buffer of the context's own; calls that
+ * overlap (two streams, two captured graphs) need workspaces of their own. */
+size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type);
+int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, void* y, int type, int M, int N, int K,
+                               int group, int scale_type, int with_zeros, void* workspace, void* stream,
+                               double* seconds);
+
+/* ---- orthogonalised updates -------------------------------------------------- */
+/* Newton-Schulz iterations on `batch` matrices g[rows][cols] of `type`, one behind the other:
+ *   x = g / (|g|_F + eps), then `steps` times  a = x x^T,  x = c0 x + (c1 a + c2 a a) x
+ * and for rows > cols the same on the transpose; out[batch][rows][cols] = x, of `type` (out == g is
+ * allowed).  With coefficients such as 3.4445, -4.7750, 2.0315 and 5 steps every singular value of g moves
+ * close to 1, which is how the Muon optimiser treats the gradient of a weight matrix
+ * (grad_w of cake_hip_linear_backward).
+ * steps >= 1.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
+ * count as they are, the result is rounded once).  Singular values start in 0..1; coefficients whose
+ * polynomial takes them beyond 1000 within `steps` are refused (CAKE_HIP_ERR_ARG).  x is kept to
+ * 2^-24 of each value and no finer than 2^-39 (for the coefficients above), so a g whose
+ * norm lies below about 1e-4 eps loses relative accuracy.  A matrix of zeros gives zeros; one that holds a NaN
+ * or an infinity gives NaN and leaves the rest of the batch alone.
+ * workspace: device memory of cake_hip_orthogonalize_workspace bytes, 256-byte aligned, or NULL for a
+ * buffer of the context's own; calls that overlap need workspaces of their own. */
+size_t cake_hip_orthogonalize_workspace(int batch, int rows, int cols);
+int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0,
+                           double c1, double c2, double eps, void* workspace, void* stream, double* seconds);
+
 /* ---- autotuner --------------------------------------------------------------- */
 /* Times macro-tile x split-K x tail-split candidates for an M x N x K product on
  * the device (synthetic operands in library memory, default stream) for at most

@@ -1,0 +1,296 @@
+"""GPU checks of the 4-bit linear layer against its definition in 64 bits.
+
+Quantising and dequantising are exact statements (codes, scales and zero points are determined), so
+their values have to be equal.  A product's bar: with S = sum_k s (code + |zero|) |x| the sum of everything that
+is added in fp32, every result is within R 2^-24 S of the 64-bit sum, R counting the roundings in a row:
+at most 16 for a block of 128 columns (four matrix instructions that round their sum of 32 products no more than
+twice, for the codes and for the column of ones, and two operations per group of 32) and 48 for the joining of
+waves and pieces and the bias; then half a step of the output's type, and half of fp16's last subnormal step."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import cake_on_cpu_amd as cake
+from cake_on_cpu_amd import _lib
+from cake_on_cpu_amd import torch_linear as tl
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _weights(N, K, group, zeros, scale_dtype, seed):
+    """codes as bytes and as numbers [N][K], scales, zero points, the values in 64 bits, and s (code + |zero|)"""
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-K // group)
+    packed = torch.randint(0, 256, (N, (K + 1) // 2), generator=g, dtype=torch.uint8)
+    s = (0.01 * torch.randn(N, groups, generator=g).exp()).to(scale_dtype)
+    z = (torch.rand(N, groups, generator=g) * 15).to(scale_dtype) if zeros else None     # no whole numbers
+    k = torch.arange(K)
+    code = ((packed[:, k // 2].int() >> (4 * (k % 2)).int()) & 15).double()
+    s64, z64 = s.double()[:, k // group], (z.double()[:, k // group] if zeros else torch.full((N, K), 8.0, dtype=torch.float64))
+    return packed, s, z, (code - z64) * s64, s64.abs() * (code + z64.abs())
+
+
+def _check(y, x, v64, mass, bias, K):
+    x64 = x.double().cpu()
+    want = x64 @ v64.t()
+    S = x64.abs() @ mass.t()
+    if bias is not None:
+        want = want + bias.double().cpu()
+        S = S + bias.double().cpu().abs()
+    R = 16 * (-(-K // 128)) + 48
+    tol = R * 2.0 ** -24 * S + 2.0 ** -40
+    if y.dtype != torch.float32:
+        tol = tol + torch.finfo(y.dtype).eps / 2 * (want.abs() + tol) + (2.0 ** -25 if y.dtype == torch.float16 else 0)
+    far = (y.double().cpu() - want).abs() - tol
+    assert y.shape == want.shape and bool((far <= 0).all()), float(far.max())
+
+
+# M, N, K: one token to many, odd sizes, a single row or column, one group, short last groups and blocks
+SHAPES = [(1, 1, 1), (1, 16, 128), (1, 17, 33), (1, 100, 1000), (1, 1024, 4096), (2, 31, 129), (3, 256, 257), (4, 40, 512), (5, 33, 640),
+          (6, 50, 300), (7, 64, 96), (10, 48, 1111), (11, 65, 256), (16, 130, 384), (17, 47, 2048), (21, 32, 500), (22, 33, 128),
+          (32, 96, 1000), (33, 70, 2111), (64, 48, 130), (65, 40, 77), (100, 111, 960), (130, 260, 520), (257, 300, 384), (600, 96, 200)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_q4_against_64_bits(shape, kind):
+    M, N, K = shape
+    for i, (group, zeros, scale) in enumerate(((32, True, "f32"), (64, False, "bf16"), (128, True, "f16"), (128, False, "f32"), (32, False, "f16"),
+                                               (64, True, "bf16"))):
+        print(f"linear_q4 M={M} N={N} K={K} {kind} group={group} zeros={zeros} scales={scale}", flush=True)
+        packed, s, z, v64, mass = _weights(N, K, group, zeros, TYPES[scale], 7 * i + M)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+        x = torch.randn(M, K, generator=torch.Generator().manual_seed(i)).to(TYPES[kind]).cuda()
+        bias = torch.randn(N, generator=torch.Generator().manual_seed(50 + i)).to(TYPES[kind]).cuda() if i % 2 else None
+        y = tl.forward_q4(x, q, bias)
+        _check(y, x, v64, mass, bias, K)
+        # the packed weights stand for the codes they were made of, bit for bit
+        assert torch.equal(tl.dequantize_q4(q).cpu(), v64.float() if not zeros else _product32(packed, s, z, K, group))
+        # and the result does not change from call to call
+        assert torch.equal(y, tl.forward_q4(x, q, bias))
+
+
+def _product32(packed, s, z, K, group):
+    k = torch.arange(K)
+    code = ((packed[:, k // 2].int() >> (4 * (k % 2)).int()) & 15).float()
+    return (code - z.float()[:, k // group]) * s.float()[:, k // group]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_of_x_off_alignment_and_guards_around_y(kind):
+    """x that starts one element behind a 16-byte border, and y inside a larger buffer that stays as it was."""
+    t = TYPES[kind]
+    for M, N, K in ((1, 33, 264), (9, 47, 1000), (70, 50, 136)):
+        packed, s, z, v64, mass = _weights(N, K, 64, True, torch.float32, M)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda(), K, 64)
+        flat = torch.randn(M * K + 1, generator=torch.Generator().manual_seed(3)).to(t).cuda()
+        x = flat[1:].view(M, K)
+        around = torch.full((M * N + 64,), 7.0, dtype=t, device="cuda")
+        y = around[32:32 + M * N].view(M, N)
+        print(f"linear_q4 unaligned M={M} N={N} K={K} {kind}", flush=True)
+        cake.linear_q4_forward(x, q, None, y, M, timed=False)
+        _check(y, x, v64, mass, None, K)
+        assert bool((around[:32] == 7).all()) and bool((around[32 + M * N:] == 7).all())
+
+
+def test_views_are_made_contiguous_and_values_of_every_size_survive():
+    N, K, M = 48, 256, 6
+    packed, s, z, v64, mass = _weights(N, K, 128, False, torch.float32, 1)
+    q = tl.pack_q4(packed.cuda(), s.cuda(), None, K, 128)
+    wide = torch.randn(K, M, generator=torch.Generator().manual_seed(3)).cuda()
+    _check(tl.forward_q4(wide.t(), q), wide.t(), v64, mass, None, K)
+    # fp32 and bf16 reach beyond fp16: nothing overflows or vanishes on the way to the matrix pipe
+    for scale in (1e-30, 1e30):
+        for t in (torch.float32, torch.bfloat16):
+            x = (torch.randn(M, K, generator=torch.Generator().manual_seed(4)) * scale).to(t)
+            want = x.double() @ v64.t()
+            tol = (16 * 2 + 48) * 2.0 ** -24 * (x.double().abs() @ mass.t()) + torch.finfo(t).eps * want.abs()
+            assert bool(((tl.forward_q4(x.cuda(), q).double().cpu() - want).abs() <= tol).all()), (scale, t)
+    # one token's NaN is that token's alone
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(5)).cuda()
+    y0 = tl.forward_q4(x, q)
+    x[2, 17] = float("nan")
+    y1 = tl.forward_q4(x, q)
+    keep = [0, 1, 3, 4, 5]
+    assert bool(torch.isnan(y1[2]).all()) and torch.equal(y1[keep], y0[keep])
+
+
+def test_empty_dimensions_and_host_operands():
+    f32 = np.float32
+    y = np.full((3, 5), np.nan, f32)
+    bias = np.arange(5, dtype=f32)
+    empty = cake.q4_of(np.zeros(16, np.uint8)[:0], 5, 0, 32, "float32", False)
+    cake.linear_q4_forward(np.zeros(1, f32), empty, bias, y, 3)          # K = 0: y = bias
+    assert np.array_equal(y, np.broadcast_to(bias, (3, 5)))
+    cake.linear_q4_forward(np.zeros(1, f32), empty, None, y, 3)
+    assert not y.any()
+    N, K, M = 70, 333, 5
+    packed, s, z, v64, mass = _weights(N, K, 32, True, torch.float32, 2)
+    q = cake.q4_pack(packed.numpy(), s.numpy(), z.numpy(), N, K, 32)
+    x = np.random.default_rng(1).standard_normal((M, K)).astype(f32)
+    y = np.full((M, N), np.nan, f32)
+    secs = cake.linear_q4_forward(x, q, None, y, M)
+    assert secs > 0
+    _check(torch.from_numpy(y), torch.from_numpy(x), v64, mass, None, K)
+    w = np.full((N, K), np.nan, f32)
+    cake.q4_dequantize(q, w)
+    assert np.array_equal(w, _product32(packed, s, z, K, 32).numpy())
+
+
+def _quantized64(w, group, zeros, scale_dtype):
+    """The definition in 64 bits: scales, zero points and the values of the codes"""
+    w = w.double()
+    N, K = w.shape
+    out = torch.empty(N, K, dtype=torch.float64)
+    for k0 in range(0, K, group):
+        run = w[:, k0:k0 + group]
+        hi, lo = run.amax(1).clamp(min=0), run.amin(1).clamp(max=0)
+        s = ((hi - lo) / 15 if zeros else torch.maximum(hi, -lo) / 7).float().to(scale_dtype).double()[:, None]
+        z = torch.where(s > 0, torch.round(-lo[:, None] / s), 8.0).clamp(0, 15) if zeros else 8.0
+        c = torch.where(s > 0, torch.round(run / s), 0.0).add(z).clamp(0, 15)
+        out[:, k0:k0 + group] = (c - z) * s
+    return out
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (16, 128), (17, 129), (5, 31), (33, 1000), (100, 4099), (257, 264), (2111, 40)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("zeros", [False, True], ids=["plain", "zeros"])
+def test_quantize_is_the_definition(shape, zeros):
+    N, K = shape
+    for i, (kind, scale, group) in enumerate((("f32", "f32", 32), ("f32", "bf16", 128), ("bf16", "f32", 64), ("f16", "f16", 32), ("bf16", "bf16", 128),
+                                              ("f16", "f32", 64))):
+        print(f"quantize N={N} K={K} {kind} scales={scale} group={group} zeros={zeros}", flush=True)
+        g = torch.Generator().manual_seed(11 + i)
+        w = torch.randn(N, K, generator=g) * 0.02
+        w[N // 2] = 0                                                       # a row of zeros
+        w[0] = w[0].abs()                                                   # a row of one sign
+        # whole numbers: quotients that are ties
+        if N > 3:
+            w[3] = torch.randint(-7, 8, (K,), generator=g) * 0.25
+        w = w.to(TYPES[kind])
+        q = tl.quantize_q4(w.cuda(), group, zeros, TYPES[scale])
+        want = _quantized64(w, group, zeros, TYPES[scale])
+        assert torch.equal(tl.dequantize_q4(q, torch.float32).cpu(), want.float())
+        for t in (torch.float16, torch.bfloat16):
+            assert torch.equal(tl.dequantize_q4(q, t).cpu(), want.float().to(t))
+
+
+def test_quantize_small_and_large_weights():
+    for scale in (1e-42, 1e-38, 1e-30, 1e30, 1e38):
+        w = (torch.randn(40, 256, generator=torch.Generator().manual_seed(1)).clamp(-2, 2) * scale).float()
+        for zeros in (False, True):
+            q = tl.quantize_q4(w.cuda(), 64, zeros, torch.float32)
+            assert torch.equal(tl.dequantize_q4(q).cpu(), _quantized64(w, 64, zeros, torch.float32).float()), (scale, zeros)
+    # a run with a NaN or an infinity comes back as such, its neighbours as they are
+    w = torch.randn(20, 256, generator=torch.Generator().manual_seed(2))
+    clean = tl.dequantize_q4(tl.quantize_q4(w.cuda(), 64)).cpu()
+    w[3, 70] = float("nan")
+    w[5, 200] = float("inf")
+    back = tl.dequantize_q4(tl.quantize_q4(w.cuda(), 64)).cpu()
+    bad = torch.zeros(20, 256, dtype=torch.bool)
+    bad[3, 64:128] = True
+    bad[5, 192:256] = True
+    assert torch.equal(back[~bad], clean[~bad]) and not bool(torch.isfinite(back[bad]).any())
+
+
+def test_gradients_of_the_layer():
+    """Input and bias gradients against the formula in 64 bits and against differences."""
+    M, N, K = 9, 50, 200
+    packed, s, z, v64, mass = _weights(N, K, 64, True, torch.float32, 3)
+    q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda(), K, 64)
+    for t in (torch.float32, torch.bfloat16):
+        x = torch.randn(M, K, generator=torch.Generator().manual_seed(1)).to(t).cuda().requires_grad_()
+        b = torch.randn(N, generator=torch.Generator().manual_seed(2)).to(t).cuda().requires_grad_()
+        gy = torch.randn(M, N, generator=torch.Generator().manual_seed(3)).to(t).cuda()
+        tl.forward_q4(x, q, b).backward(gy)
+        g64 = gy.double().cpu()
+        # N products and the rounding of each weight to 32 bits, then the type
+        tol = (N + 8) * 2.0 ** -24 * (g64.abs() @ v64.abs()) + torch.finfo(t).eps / 2 * (g64 @ v64).abs() * 1.01
+        assert bool(((x.grad.double().cpu() - g64 @ v64).abs() <= tol).all())
+        tol = M * 2.0 ** -24 * g64.abs().sum(0) + torch.finfo(t).eps / 2 * g64.sum(0).abs() * 1.01
+        assert bool(((b.grad.double().cpu() - g64.sum(0)).abs() <= tol).all())
+    # y is linear in x: a difference is exact up to the bar of the two products
+    x0 = torch.randn(M, K, generator=torch.Generator().manual_seed(4))
+    d = torch.randn(M, K, generator=torch.Generator().manual_seed(5))
+    gy = torch.randn(M, N, generator=torch.Generator().manual_seed(6))
+    x = x0.cuda().requires_grad_()
+    tl.forward_q4(x, q).backward(gy.cuda())
+    up, down = tl.forward_q4((x0 + d).cuda(), q), tl.forward_q4((x0 - d).cuda(), q)
+    slope = float(((up - down).double().cpu() * gy.double()).sum() / 2)
+    want = float((x.grad.double().cpu() * d.double()).sum())
+    bar = (16 * 2 + 48) * 2.0 ** -24 * float(((x0.abs() + d.abs()).double() @ mass.t() * gy.double().abs()).sum()) * 2
+    assert abs(slope - want) <= bar
+
+
+def test_layer_modules_round_trip():
+    torch.manual_seed(0)
+    layer = tl.cake_linear(300, 130).cuda()
+    held = tl.cake_linear_q4.of(layer, group=64, zeros=True)
+    x = torch.randn(2, 7, 300, device="cuda")
+    y = held(x)
+    assert y.shape == (2, 7, 130)
+    w = tl.dequantize_q4(held.weight_q4).double().cpu()
+    want = x.double().cpu() @ w.t() + layer.bias.double().cpu()
+    assert float((y.double().cpu() - want).abs().max()) <= (16 * 3 + 48) * 2.0 ** -24 * 300 * 4 * float(w.abs().max()) * 15
+    other = tl.cake_linear_q4.of(tl.cake_linear(300, 130).cuda(), group=64, zeros=True)
+    other.load_state_dict(held.state_dict())
+    assert torch.equal(other(x), y)
+    assert held(x.bfloat16()).dtype == torch.bfloat16
+    cpu = tl.cake_linear_q4(cake.q4_of(held.packed.cpu(), 130, 300, 64, torch.bfloat16, True), held.bias.cpu())
+    assert torch.equal(cpu(x.cpu()), y.cpu())
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 200])
+def test_captured_calls_on_two_graphs_and_streams(M):
+    """Two graphs captured from the same weights replay side by side on streams of their own, with eager
+    calls between, and every replay gives the eager result for the inputs of that moment."""
+    N, K = 520, 1500
+    packed, s, z, _, _ = _weights(N, K, 32, True, torch.float16, 5)
+    q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda(), K, 32)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    xs = [torch.randn(M, K, device="cuda", generator=gen) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for x, st in zip(xs, streams):
+        with torch.cuda.stream(st):
+            tl.forward_q4(x, q)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, st in zip(xs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(tl.forward_q4(x, q))
+        graphs.append(g)
+    for replay in range(4):
+        for x in xs:
+            x.copy_(torch.randn(M, K, device="cuda", generator=gen))
+        want = [tl.forward_q4(x, q) for x in xs]
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), replay
+
+
+def test_refusals_on_the_device():
+    N, K = 32, 128
+    q = tl.quantize_q4(torch.ones(N, K, device="cuda"), 128)
+    x, y = torch.ones(2, K, device="cuda"), torch.full((2, N), 7.0, device="cuda")
+    lib = cake.load()
+    off = torch.zeros(q.data.numel() + 16, dtype=torch.uint8, device="cuda")[4:]
+    st = lib.cake_hip_linear_q4_forward(x.data_ptr(), off.data_ptr(), None, y.data_ptr(), _lib.F32, 2, N, K, 128, _lib.BF16, 0, None, None, None)
+    assert st == _lib.ERR_ARG and b"aligned" in lib.cake_hip_last_error()
+    assert lib.cake_hip_q4_quantize(x.data_ptr(), _lib.F32, off.data_ptr(), 2, K, 128, _lib.BF16, 0, None, None) == _lib.ERR_ARG
+    host = np.zeros(1 << 16, np.uint8)
+    st = lib.cake_hip_linear_q4_forward(x.data_ptr(), q.data.data_ptr(), None, y.data_ptr(), _lib.F32, 2, N, K, 128, _lib.BF16, 0,
+                                        off.data_ptr(), None, None)
+    assert st == _lib.ERR_ARG
+    with pytest.raises(ValueError):
+        tl.forward_q4(x.cpu(), q)
+    torch.cuda.synchronize()
+    assert bool((y == 7).all())
+    del host
