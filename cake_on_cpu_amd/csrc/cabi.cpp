@@ -2317,8 +2317,8 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
     return stage_out(yo, stream);
 }
 
-// How far a singular value from [0, 1] and the polynomial that multiplies it can get in `steps`
-// iterations, and from that the powers of two under which x, a = x x^T and b = c0 + c1 a + c2 a a stay
+// How far a singular value from [0, 1] and the matrix that multiplies it can get in `steps`
+// iterations, and from that the powers of two under which x, a = x x^T and b = c1 a + c2 a a stay
 // below fp16's 65504 (no entry of a matrix exceeds its largest singular value).
 static int orthogonalize_scales(int steps, double c0, double c1, double c2, OrthogonalizeScales* out)
 {
@@ -2326,10 +2326,11 @@ static int orthogonalize_scales(int steps, double c0, double c1, double c2, Orth
     for (int i = 0; i < steps; ++i) {
         const double end = u * u;
         auto poly = [&](double s) { return fabs(c0 + s * (c1 + s * c2)); };
-        double b = fmax(poly(0), poly(end));
-        if (c2 != 0) {   // the polynomial's own vertex
+        auto rest = [&](double s) { return fabs(s * (c1 + s * c2)); };
+        double b = rest(end);
+        if (c2 != 0) {   // the parabola's own vertex
             const double v = -c1 / (2 * c2);
-            if (v > 0 && v < end) b = fmax(b, poly(v));
+            if (v > 0 && v < end) b = fmax(b, rest(v));
         }
         highest = fmax(highest, b);
         double next = u * poly(end);

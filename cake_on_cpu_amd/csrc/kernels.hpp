@@ -291,8 +291,8 @@ size_t linear_q4_workspace(int M, int N, int K, int type);
 struct OrthogonalizeLayout {
     int m, n;                     // the shorter and the longer side
     int mb, nb;                   // in blocks of 16, even
-    size_t x_halves, a_halves;    // of one matrix of the batch
-    size_t x, xt0, xt1, a, b, partial, bytes;
+    size_t x_halves, a_halves;    // of one matrix of the batch; the carried x has x_halves / 2 floats
+    size_t x, xt0, xt1, a, b, partial, carried, slices, bytes;
 };
 // powers of two that the values of x, a and b are multiplied by where they are kept
 struct OrthogonalizeScales {

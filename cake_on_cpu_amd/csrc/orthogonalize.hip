@@ -1,5 +1,5 @@
 // orthogonalize.hip -- Newton-Schulz iterations on a batch of matrices:
-//   x = g / (|g|_F + eps), then steps times  a = x x^T,  b = c0 I + c1 a + c2 a a,  x = b x
+//   x = g / (|g|_F + eps), then steps times  a = x x^T,  b = c1 a + c2 a a,  x = c0 x + b x
 // (for more rows than columns on the transpose).
 //
 // All products run on the 16-bit matrix pipe at 32-bit accuracy.  A value v is kept as two fp16
@@ -9,8 +9,12 @@
 // hi hi + hi lo + lo hi -- three matrix instructions where the fp32 ones, at a sixteenth of the rate,
 // would take the time of sixteen -- summed in 32 bits; lo lo is below 2^-24 of the product.  The
 // floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39 of the largest a value can be.
+// x itself is carried from step to step in fp32 beside its pairs, and b is kept without c0 I: early
+// steps are little more than x = c0 x, and what is lost of a small singular value there is
+// enlarged by every later step (on a 1024 x 1024 gradient the final error is 4e-7 with the carried x and
+// 9e-7 with x kept as pairs alone; fp32 products give 1.3e-6).
 //
-// a, a a and b are symmetric: only tiles on and above the diagonal are computed and written twice.
+// a and a a are symmetric: only tiles on and above the diagonal are computed and written twice.
 //
 // Operand form.  Every product here is P . Q^T with both operands read along k, so a matrix is kept
 // as blocks of 16 rows x 32 columns, [column block][row block][hi, lo], and a block is the 1 KB that
@@ -20,6 +24,9 @@
 // to multiples of 32; x is kept along its columns and, for the product b x, along its rows.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "kernels.hpp"
 #include "low_bits.hpp"
 
@@ -28,7 +35,7 @@ namespace cake {
 namespace {
 
 constexpr int BLOCK = 512;        // halves of one part of a 16 x 32 block
-enum { NORM_CHUNKS = 512 };
+enum { NORM_CHUNKS = 512, MAX_SLICES = 32 };
 
 // Element (row, col) of a matrix of row_blocks blocks of 16 rows: halves from its start to the hi part;
 // the lo part is BLOCK further.
@@ -36,6 +43,9 @@ __device__ __forceinline__ size_t pair_at(int row, int col, int row_blocks)
 {
     return ((size_t)(col >> 5) * row_blocks + (row >> 4)) * (2 * BLOCK) + ((row & 15) + ((col >> 3) & 3) * 16) * 8 + (col & 7);
 }
+
+// The carried x: blocks of 16 x 16 floats, four a lane as a product's results come out of the matrix pipe.
+__device__ __forceinline__ size_t carried_at(int bi, int bj, int row_blocks) { return ((size_t)bj * row_blocks + bi) * 256; }
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo)
 {
@@ -62,8 +72,8 @@ __global__ __launch_bounds__(256) void norm_partial_kernel(const void* __restric
 // x0 = g / (norm + eps) in both orders.  m <= n are x's sides; `tall`: g is n x m.  A workgroup takes
 // 64 x 64 of x through LDS, so that g is read and the blocks are written in whole lines.
 __global__ __launch_bounds__(256) void normalize_kernel(const void* __restrict__ g, int type, const double* __restrict__ partial, int chunks,
-                                                        double eps, float up, _Float16* __restrict__ x, _Float16* __restrict__ xt, int m,
-                                                        int n, int mb, int nb, bool tall, size_t x_stride)
+                                                        double eps, float up, _Float16* __restrict__ x, _Float16* __restrict__ xt,
+                                                        float* __restrict__ carried, int m, int n, int mb, int nb, bool tall, size_t x_stride)
 {
     __shared__ float tile[64][65];
     __shared__ double red[4];
@@ -80,12 +90,20 @@ __global__ __launch_bounds__(256) void normalize_kernel(const void* __restrict__
     for (int r = tid >> 6; r < 64; r += 4) {
         const int i = tall ? i0 + lane : i0 + r, j = tall ? j0 + r : j0 + lane;
         float v = 0;
-        if (i < m && j < n) v = (float)((double)load_as_float(g, base + (tall ? (size_t)j * m + i : (size_t)i * n + j), type) * by) * up;
+        if (i < m && j < n) v = (float)((double)load_as_float(g, base + (tall ? (size_t)j * m + i : (size_t)i * n + j), type) * by);
         tile[i - i0][j - j0] = v;
     }
     __syncthreads();
     x += blockIdx.z * x_stride;
     xt += blockIdx.z * x_stride;
+    carried += blockIdx.z * (x_stride / 2);
+    for (int u = tid >> 6; u < 16; u += 4) {
+        const int bi = i0 / 16 + (u >> 2), bj = j0 / 16 + (u & 3);
+        if (bi >= mb || bj >= nb) continue;
+        const int row = (u >> 2) * 16 + (lane >> 4) * 4, col = (u & 3) * 16 + (lane & 15);
+        *reinterpret_cast<floatx4*>(carried + carried_at(bi, bj, mb) + lane * 4) =
+            floatx4{tile[row][col], tile[row + 1][col], tile[row + 2][col], tile[row + 3][col]};
+    }
     // 4 row blocks x 2 column blocks of x, and as many of its transpose
     for (int u = tid >> 6; u < 16; u += 4) {
         const bool turned = u >= 8;
@@ -95,7 +113,7 @@ __global__ __launch_bounds__(256) void normalize_kernel(const void* __restrict__
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             _Float16 h, l;
-            split(turned ? tile[col + e][row] : tile[row][col + e], h, l);
+            split((turned ? tile[col + e][row] : tile[row][col + e]) * up, h, l);
             hi[e] = h;
             lo[e] = l;
         }
@@ -108,25 +126,98 @@ __global__ __launch_bounds__(256) void normalize_kernel(const void* __restrict__
     }
 }
 
-enum { GRAM = 0, POLYNOMIAL = 1, APPLY = 2 };
+enum { GRAM = 0, POLYNOMIAL = 1, APPLY = 2, FINISH = 3 };   // FINISH: the last step's APPLY, into the caller's matrix
 
 struct PairGemm {
     const _Float16* p;        // rows i
     const _Float16* q;        // rows j
     const _Float16* a;        // POLYNOMIAL: a itself
-    _Float16* out;            // GRAM, POLYNOMIAL: the symmetric result; APPLY: x (or nullptr on the last step)
+    float* carried;           // APPLY, FINISH
+    _Float16* out;            // GRAM, POLYNOMIAL: the symmetric result; APPLY: x
     _Float16* out_t;          // APPLY: its transpose
-    void* result;             // APPLY, last step: the caller's matrix
+    void* result;             // FINISH
+    float* partial;           // sums of K slices, or nullptr
     int type;                 // of the result
     bool tall;
     int mi, mj;               // the result's real sides
     int ib, jb, kb;           // blocks of 16 rows of either operand, of 32 columns
-    int tiles_i, tiles_j;
+    int tiles_i, tiles_j, tiles;
+    int slices;               // workgroups along k of a tile
     size_t p_stride, q_stride, a_stride, out_stride, result_stride;   // from one matrix of the batch to the next
     float unscale;            // of the accumulated product
     float c0, c1, c2;
     float a_unscale, up;      // of a's parts; 2^e of the result
 };
+
+// Tile number -> (ti, tj): all of them, ti fastest (workgroups that run together share columns of x),
+// or of a symmetric result those with ti <= tj, column by column.
+template <int MODE>
+__device__ __forceinline__ void tile_of(int id, int tiles_i, int& ti, int& tj)
+{
+    if (MODE >= APPLY) {
+        ti = id % tiles_i;
+        tj = id / tiles_i;
+    } else {
+        tj = (int)((__builtin_sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
+        while (tj * (tj + 1) / 2 > id) --tj;
+        while ((tj + 1) * (tj + 2) / 2 <= id) ++tj;
+        ti = id - tj * (tj + 1) / 2;
+    }
+}
+
+// What becomes of one block of 16 x 16 sums: a lane holds column lane & 15 in four consecutive rows.
+template <int MODE>
+__device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, int bj, bool mirror, floatx4 v, int lane)
+{
+    const int row = bi * 16 + (lane >> 4) * 4, c = bj * 16 + (lane & 15);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] *= g.unscale;
+    const size_t turned = pair_at(c, row, g.jb);   // (column, rows): 4 consecutive halves
+    if (MODE >= APPLY) {
+        floatx4* x = reinterpret_cast<floatx4*>(g.carried + z * (g.out_stride / 2) + carried_at(bi, bj, g.ib) + lane * 4);
+        const floatx4 was = *x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(g.c0, was[r], v[r]);
+        if (MODE == APPLY) *x = v;
+    }
+    if (MODE == FINISH) {
+        const size_t base = z * g.result_stride;
+        if (c < g.mj) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row + r < g.mi)
+                    store_from_float(g.result, base + (g.tall ? (size_t)c * g.mi + row + r : (size_t)(row + r) * g.mj + c), g.type, v[r]);
+        }
+        return;
+    }
+    if (MODE == POLYNOMIAL) {
+        const _Float16* a = g.a + z * g.a_stride + turned;
+        const f16x4 ah = *reinterpret_cast<const f16x4*>(a), al = *reinterpret_cast<const f16x4*>(a + BLOCK);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = g.c2 * v[r] + g.c1 * (((float)ah[r] + (float)al[r]) * g.a_unscale);
+    }
+    f16x4 hi, lo;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        _Float16 h, l;
+        split(v[r] * g.up, h, l);
+        hi[r] = h;
+        lo[r] = l;
+    }
+    _Float16* out = g.out + z * g.out_stride;
+    _Float16* to = (MODE == APPLY ? g.out_t + z * g.out_stride : out) + turned;
+    *reinterpret_cast<f16x4*>(to) = hi;
+    *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
+    // and in the other order: x itself, or the mirrored tile of a symmetric result
+    if (MODE == APPLY || mirror) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            _Float16* also = out + pair_at(row + r, c, g.ib);
+            also[0] = hi[r];
+            also[BLOCK] = lo[r];
+        }
+    }
+}
 
 // out = P . Q^T over WI x WJ waves of TI x TJ blocks of 16 x 16 each.  A stage is one column block (32
 // of k) of both operands; the next one travels to registers while this one is multiplied and is
@@ -136,50 +227,44 @@ __global__ __launch_bounds__(64 * WI * WJ) void pair_gemm_kernel(PairGemm g)
 {
     constexpr int BI = WI * TI, BJ = WJ * TJ;                  // blocks per tile
     constexpr int STAGE = (BI + BJ) * 2 * BLOCK;               // halves
-    constexpr int LOADS = (BI + BJ) * 2 / (WI * WJ);           // parts of 1 KB per wave
-    static_assert((BI + BJ) * 2 % (WI * WJ) == 0, "parts must divide among the waves");
+    constexpr int WAVES = WI * WJ;
+    constexpr int LOADS = (BI + BJ) * 2 / WAVES;               // parts of 1 KB per wave
+    constexpr int P_LOADS = BI * 2 / WAVES;
+    static_assert(BI * 2 % WAVES == 0 && BJ * 2 % WAVES == 0, "either operand's parts must divide among the waves");
     extern __shared__ __align__(16) _Float16 stage[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave / WJ, wj = wave % WJ;
 
     int ti, tj;
-    if (MODE == APPLY) {
-        ti = blockIdx.x % g.tiles_i;
-        tj = blockIdx.x / g.tiles_i;
-    } else {   // tiles with ti <= tj, column by column
-        const int id = blockIdx.x;
-        tj = (int)((__builtin_sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
-        while (tj * (tj + 1) / 2 > id) --tj;
-        while ((tj + 1) * (tj + 2) / 2 <= id) ++tj;
-        ti = id - tj * (tj + 1) / 2;
-    }
+    const int slice = blockIdx.x / g.tiles, tile = blockIdx.x - slice * g.tiles;
+    tile_of<MODE>(tile, g.tiles_i, ti, tj);
+    const int k0 = (int)((long long)g.kb * slice / g.slices), k1 = (int)((long long)g.kb * (slice + 1) / g.slices);
     const _Float16* p = g.p + blockIdx.z * g.p_stride;
     const _Float16* q = g.q + blockIdx.z * g.q_stride;
 
     // the parts this wave fetches: block t of the tile (P's, then Q's), hi or lo; rows past the
     // operand's last block repeat that block, and their results are not stored
-    const _Float16* from[LOADS];
-    size_t step[LOADS];
+    const char* from_p = reinterpret_cast<const char*>(p);     // the same for every lane: addresses are scalars
+    const char* from_q = reinterpret_cast<const char*>(q);
+    const size_t step_p = (size_t)g.ib * 4 * BLOCK, step_q = (size_t)g.jb * 4 * BLOCK;
+    from_p += k0 * step_p;
+    from_q += k0 * step_q;
+    unsigned at_part[LOADS];
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
-        const int part = wave * LOADS + l, t = part >> 1;
-        const bool of_p = t < BI;
-        const int block = of_p ? min(ti * BI + t, g.ib - 1) : min(tj * BJ + t - BI, g.jb - 1);
-        from[l] = (of_p ? p : q) + (size_t)block * 2 * BLOCK + (part & 1) * BLOCK + lane * 8;
-        step[l] = (size_t)(of_p ? g.ib : g.jb) * 2 * BLOCK;
+        const int part = l * WAVES + wave, t = part >> 1;
+        const int block = l < P_LOADS ? min(ti * BI + t, g.ib - 1) : min(tj * BJ + t - BI, g.jb - 1);
+        at_part[l] = (unsigned)block * 4 * BLOCK + (part & 1) * 2 * BLOCK + lane * 16;
     }
     f16x8 next[LOADS];
-    auto fetch = [&]() {
-#pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            next[l] = *reinterpret_cast<const f16x8*>(from[l]);
-            from[l] += step[l];
-        }
+    auto fetch = [&](int l) { next[l] = *reinterpret_cast<const f16x8*>((l < P_LOADS ? from_p : from_q) + at_part[l]); };
+    auto put = [&](int l, int half) {
+        *reinterpret_cast<f16x8*>(stage + half * STAGE + (l * WAVES + wave) * BLOCK + lane * 8) = next[l];
     };
-    auto put = [&](int half) {
-#pragma unroll
-        for (int l = 0; l < LOADS; ++l)
-            *reinterpret_cast<f16x8*>(stage + half * STAGE + (wave * LOADS + l) * BLOCK + lane * 8) = next[l];
+    // to the column block `of`; past the last one the last is fetched again, and nobody reads it
+    auto advance = [&](int of) {
+        from_p += of < k1 ? step_p : 0;
+        from_q += of < k1 ? step_q : 0;
     };
 
     floatx4 acc[TI][TJ];
@@ -187,104 +272,182 @@ __global__ __launch_bounds__(64 * WI * WJ) void pair_gemm_kernel(PairGemm g)
     for (int i = 0; i < TI; ++i)
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[i][j] = floatx4{0, 0, 0, 0};
-    fetch();
-    put(0);
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) fetch(l);
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) put(l, 0);
+    advance(k0 + 1);
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) fetch(l);
     __syncthreads();
-    for (int k = 0; k < g.kb; ++k) {
-        if (k + 1 < g.kb) fetch();
-        const _Float16* at = stage + (k & 1) * STAGE + lane * 8;
+    for (int k = k0; k < k1; ++k) {
+        const int half = (k - k0) & 1;
+        const _Float16* at = stage + half * STAGE + lane * 8;
         const _Float16* at_p = at + wi * TI * 2 * BLOCK;
         const _Float16* at_q = at + (BI + wj * TJ) * 2 * BLOCK;
-        f16x8 qh[TJ], ql[TJ];
+        advance(k + 2);
+        f16x8 qh[TJ], ql[TJ], ph[2], pl[2];
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
             qh[j] = *reinterpret_cast<const f16x8*>(at_q + j * 2 * BLOCK);
             ql[j] = *reinterpret_cast<const f16x8*>(at_q + j * 2 * BLOCK + BLOCK);
         }
+        ph[0] = *reinterpret_cast<const f16x8*>(at_p);
+        pl[0] = *reinterpret_cast<const f16x8*>(at_p + BLOCK);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
-            const f16x8 ph = *reinterpret_cast<const f16x8*>(at_p + i * 2 * BLOCK);
-            const f16x8 pl = *reinterpret_cast<const f16x8*>(at_p + i * 2 * BLOCK + BLOCK);
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh[j], acc[i][j], 0, 0, 0);
+            const int now = i & 1;
+            if (i + 1 < TI) {
+                ph[now ^ 1] = *reinterpret_cast<const f16x8*>(at_p + (i + 1) * 2 * BLOCK);
+                pl[now ^ 1] = *reinterpret_cast<const f16x8*>(at_p + (i + 1) * 2 * BLOCK + BLOCK);
             }
+            // this row of blocks' share of the next stage: out of the registers, and the stage after it in
+#pragma unroll
+            for (int l = i * LOADS / TI; l < (i + 1) * LOADS / TI; ++l) {
+                put(l, half ^ 1);
+                fetch(l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[now], qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[now], ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[now], qh[j], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (k + 1 < g.kb) put((k + 1) & 1);
         __syncthreads();
     }
 
-    // a lane holds column col of a block in four consecutive rows
-    const int col = lane & 15, row4 = (lane >> 4) * 4;
-    _Float16* out = g.out ? g.out + blockIdx.z * g.out_stride : nullptr;
+    if (g.partial) {
+        float* to = g.partial + (((size_t)blockIdx.z * gridDim.x + blockIdx.x) * (BI * BJ)) * 256 + lane * 4;
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) *reinterpret_cast<floatx4*>(to + ((wi * TI + i) * BJ + wj * TJ + j) * 256) = acc[i][j];
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
         const int bi = ti * BI + wi * TI + i;
-        if (bi >= g.ib) continue;
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
             const int bj = tj * BJ + wj * TJ + j;
-            if (bj >= g.jb) continue;
-            const int row = bi * 16 + row4, c = bj * 16 + col;
-            floatx4 v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * g.unscale;
-            if (MODE == APPLY && !out) {
-                const size_t base = blockIdx.z * g.result_stride;
-                if (c < g.mj) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (row + r < g.mi)
-                            store_from_float(g.result, base + (g.tall ? (size_t)c * g.mi + row + r : (size_t)(row + r) * g.mj + c), g.type, v[r]);
-                }
-                continue;
-            }
-            const size_t turned = pair_at(c, row, g.jb);   // (column, rows): 4 consecutive halves
-            if (MODE == POLYNOMIAL) {
-                const _Float16* a = g.a + blockIdx.z * g.a_stride + turned;
-                const f16x4 ah = *reinterpret_cast<const f16x4*>(a), al = *reinterpret_cast<const f16x4*>(a + BLOCK);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float av = ((float)ah[r] + (float)al[r]) * g.a_unscale;
-                    v[r] = g.c2 * v[r] + (g.c1 * av + (row + r == c ? g.c0 : 0.f));
-                }
-            }
-            f16x4 hi, lo;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                _Float16 h, l;
-                split(v[r] * g.up, h, l);
-                hi[r] = h;
-                lo[r] = l;
-            }
-            _Float16* to = (MODE == APPLY ? g.out_t + blockIdx.z * g.out_stride : out) + turned;
-            *reinterpret_cast<f16x4*>(to) = hi;
-            *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
-            // and in the other order: x itself, or the mirrored tile of a symmetric result
-            if (MODE == APPLY || ti != tj) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    _Float16* also = out + pair_at(row + r, c, g.ib);
-                    also[0] = hi[r];
-                    also[BLOCK] = lo[r];
-                }
-            }
+            if (bi < g.ib && bj < g.jb) finish_block<MODE>(g, blockIdx.z, bi, bj, ti != tj, acc[i][j], lane);
         }
     }
 }
 
+// The K slices of every tile added up in order, a wave per block.
 template <int MODE>
-hipError_t pair_gemm(PairGemm g, int batch, hipStream_t stream)
+__global__ __launch_bounds__(256) void join_slices_kernel(PairGemm g, int tile_blocks)
 {
-    constexpr int W = 2, T = 4;
-    g.tiles_i = (g.ib + W * T - 1) / (W * T);
-    g.tiles_j = (g.jb + W * T - 1) / (W * T);
-    const int tiles = MODE == APPLY ? g.tiles_i * g.tiles_j : g.tiles_i * (g.tiles_i + 1) / 2;
-    const size_t lds = (size_t)2 * 2 * W * T * 2 * BLOCK * sizeof(_Float16);
-    pair_gemm_kernel<MODE, W, W, T, T><<<dim3(tiles, 1, batch), dim3(64 * W * W), lds, stream>>>(g);
+    const int lane = threadIdx.x & 63;
+    const int per_tile = tile_blocks * tile_blocks;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int tile = unit / per_tile, block = unit - tile * per_tile;
+    if (tile >= g.tiles) return;
+    int ti, tj;
+    tile_of<MODE>(tile, g.tiles_i, ti, tj);
+    const int bi = ti * tile_blocks + block / tile_blocks, bj = tj * tile_blocks + block % tile_blocks;
+    if (bi >= g.ib || bj >= g.jb) return;
+    const size_t step = (size_t)g.tiles * per_tile * 256;
+    const float* from = g.partial + (size_t)blockIdx.z * g.slices * step + ((size_t)tile * per_tile + block) * 256 + lane * 4;
+    floatx4 v = *reinterpret_cast<const floatx4*>(from);
+    for (int s = 1; s < g.slices; ++s) v += *reinterpret_cast<const floatx4*>(from + s * step);
+    finish_block<MODE>(g, blockIdx.z, bi, bj, ti != tj, v, lane);
+}
+
+// The four tiles, and what a stage of 32 columns and a tile's beginning and end take in microseconds
+// (measured on sides of 1024 to 4096): `alone` with one workgroup on a compute unit, `full`
+// with as many as fit.
+struct TileCost {
+    int blocks, resident;
+    float alone, full;
+};
+constexpr TileCost TILES[] = {{4, 4, 0.47f, 0.95f}, {8, 2, 0.75f, 1.35f}, {12, 1, 1.42f, 1.42f}, {16, 1, 2.3f, 2.3f}};
+// The device's compute units; a number of this file, so that the size of the workspace and the order of
+// the sums follow from the sizes alone.
+constexpr int CUS = 256;
+struct TileChoice {
+    int which, slices;
+};
+
+int tile_count(int blocks, int ib, int jb, bool symmetric)
+{
+    const int i = (ib + blocks - 1) / blocks, j = (jb + blocks - 1) / blocks;
+    return symmetric ? i * (i + 1) / 2 : i * j;
+}
+
+// The tile and the number of K slices with the least estimated time.  Slices give a result of few
+// tiles to the whole device, at the price of a pass over the partial sums.
+TileChoice choose_tile(int ib, int jb, int kb, bool symmetric, int batch)
+{
+    TileChoice best{0, 1};
+    float least = 1e30f;
+    for (int w = 0; w < 4; ++w) {
+        const TileCost& t = TILES[w];
+        const float tiles = (float)tile_count(t.blocks, ib, jb, symmetric) * batch;
+        for (int s = 1; s <= MAX_SLICES && s <= kb; ++s) {
+            const float groups = tiles * s;
+            if (s > 1 && groups > CUS * t.resident) break;
+            const float rounds = ceilf(groups / (CUS * t.resident));
+            const float stage = groups <= CUS ? t.alone : t.full;
+            float us = 3.f + rounds * (stage * ((kb + s - 1) / s) + 3.f);
+            // partial sums out and back at about 3 TB/s, and a launch
+            if (s > 1) us += 4.f + groups * t.blocks * t.blocks * 2048 / 3e6f;
+            if (us < least) {
+                least = us;
+                best = {w, s};
+            }
+        }
+    }
+    return best;
+}
+
+template <int MODE, int WI, int WJ, int TI, int TJ>
+hipError_t pair_gemm_on(PairGemm g, int batch, hipStream_t stream)
+{
+    static_assert(WI * TI == WJ * TJ, "square tiles");
+    constexpr int BLOCKS = WI * TI;
+    g.tiles_i = (g.ib + BLOCKS - 1) / BLOCKS;
+    g.tiles_j = (g.jb + BLOCKS - 1) / BLOCKS;
+    g.tiles = tile_count(BLOCKS, g.ib, g.jb, MODE < APPLY);
+    constexpr size_t LDS = (size_t)2 * 2 * BLOCKS * 2 * BLOCK * sizeof(_Float16);
+    auto kernel = &pair_gemm_kernel<MODE, WI, WJ, TI, TJ>;
+    if (LDS > 64 * 1024) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<dim3(g.tiles * g.slices, 1, batch), dim3(64 * WI * WJ), LDS, stream>>>(g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || g.slices == 1) return e;
+    join_slices_kernel<MODE><<<dim3((unsigned)((size_t)g.tiles * BLOCKS * BLOCKS + 3) / 4, 1, batch), 256, 0, stream>>>(g, BLOCKS);
     return hipGetLastError();
+}
+
+template <int MODE>
+hipError_t pair_gemm(PairGemm g, int batch, float* partial, hipStream_t stream)
+{
+    const TileChoice t = choose_tile(g.ib, g.jb, g.kb, MODE < APPLY, batch);
+    g.slices = t.slices;
+    g.partial = t.slices > 1 ? partial : nullptr;
+    switch (t.which) {
+    case 0: return pair_gemm_on<MODE, 2, 2, 2, 2>(g, batch, stream);
+    case 1: return pair_gemm_on<MODE, 2, 2, 4, 4>(g, batch, stream);
+    case 2: return pair_gemm_on<MODE, 2, 4, 6, 3>(g, batch, stream);
+    default: return pair_gemm_on<MODE, 2, 4, 8, 4>(g, batch, stream);
+    }
+}
+
+// floats of partial sums that the choice above asks for
+size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
+{
+    const TileChoice t = choose_tile(ib, jb, kb, symmetric, batch);
+    if (t.slices == 1) return 0;
+    const int blocks = TILES[t.which].blocks;
+    return (size_t)tile_count(blocks, ib, jb, symmetric) * t.slices * batch * blocks * blocks * 256;
 }
 
 }  // namespace
@@ -304,7 +467,11 @@ OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols)
     l.a = l.xt1 + (size_t)batch * l.x_halves * 2;
     l.b = l.a + (size_t)batch * l.a_halves * 2;
     l.partial = l.b + (size_t)batch * l.a_halves * 2;
-    l.bytes = l.partial + (size_t)batch * NORM_CHUNKS * sizeof(double);
+    l.carried = l.partial + (size_t)batch * NORM_CHUNKS * sizeof(double);
+    l.slices = l.carried + (size_t)batch * l.x_halves * 2;
+    const size_t floats[3] = {slice_floats(l.mb, l.mb, l.nb / 2, true, batch), slice_floats(l.mb, l.mb, l.mb / 2, true, batch),
+                              slice_floats(l.mb, l.nb, l.mb / 2, false, batch)};
+    l.bytes = l.slices + std::max(floats[0], std::max(floats[1], floats[2])) * sizeof(float);
     return l;
 }
 
@@ -318,6 +485,8 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     _Float16* a = reinterpret_cast<_Float16*>(ws + l.a);
     _Float16* b = reinterpret_cast<_Float16*>(ws + l.b);
     double* partial = reinterpret_cast<double*>(ws + l.partial);
+    float* carried = reinterpret_cast<float*>(ws + l.carried);
+    float* slices = reinterpret_cast<float*>(ws + l.slices);
     const size_t values = (size_t)l.m * l.n;
     const bool tall = rows > cols;
     const size_t want = (values + 8191) / 8192;
@@ -326,8 +495,8 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const float up_x = ldexpf(1.f, sc.ex), up_a = ldexpf(1.f, sc.ea), up_b = ldexpf(1.f, sc.eb);
-    normalize_kernel<<<dim3((l.nb + 3) / 4, (l.mb + 3) / 4, batch), 256, 0, stream>>>(g, type, partial, chunks, eps, up_x, x, xt[0], l.m, l.n,
-                                                                                     l.mb, l.nb, tall, l.x_halves);
+    normalize_kernel<<<dim3((l.nb + 3) / 4, (l.mb + 3) / 4, batch), 256, 0, stream>>>(g, type, partial, chunks, eps, up_x, x, xt[0], carried, l.m,
+                                                                                     l.n, l.mb, l.nb, tall, l.x_halves);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     for (int s = 0; s < steps; ++s) {
         PairGemm k{};
@@ -340,7 +509,7 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
         k.out_stride = l.a_halves;
         k.unscale = 1.f / (up_x * up_x);
         k.up = up_a;
-        if ((e = pair_gemm<GRAM>(k, batch, stream)) != hipSuccess) return e;
+        if ((e = pair_gemm<GRAM>(k, batch, slices, stream)) != hipSuccess) return e;
         k.p = k.q = k.a = a;
         k.out = b;
         k.kb = l.mb / 2;
@@ -351,11 +520,12 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
         k.c0 = (float)c0;
         k.c1 = (float)c1;
         k.c2 = (float)c2;
-        if ((e = pair_gemm<POLYNOMIAL>(k, batch, stream)) != hipSuccess) return e;
+        if ((e = pair_gemm<POLYNOMIAL>(k, batch, slices, stream)) != hipSuccess) return e;
         const bool last = s == steps - 1;
         k.p = b;
         k.q = xt[s & 1];
-        k.out = last ? nullptr : x;
+        k.carried = carried;
+        k.out = x;
         k.out_t = xt[(s & 1) ^ 1];
         k.result = out;
         k.type = type;
@@ -366,7 +536,8 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
         k.result_stride = values;
         k.unscale = 1.f / (up_b * up_x);
         k.up = up_x;
-        if ((e = pair_gemm<APPLY>(k, batch, stream)) != hipSuccess) return e;
+        e = last ? pair_gemm<FINISH>(k, batch, slices, stream) : pair_gemm<APPLY>(k, batch, slices, stream);
+        if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
