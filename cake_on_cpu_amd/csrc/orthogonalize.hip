@@ -9,10 +9,10 @@
 // hi hi + hi lo + lo hi -- three matrix instructions where the fp32 ones, at a sixteenth of the rate,
 // would take the time of sixteen -- summed in 32 bits; lo lo is below 2^-24 of the product.  The
 // floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39 of the largest a value can be.
-// x itself is carried from step to step in fp32 beside its pairs, and b is kept without c0 I: early
-// steps are little more than x = c0 x, and what is lost of a small singular value there is
-// enlarged by every later step (on a 1024 x 1024 gradient the final error is 4e-7 with the carried x and
-// 9e-7 with x kept as pairs alone; fp32 products give 1.3e-6).
+// b is kept without c0 I, and while four or more steps follow x is carried in fp32 beside its
+// pairs: early steps are little more than x = c0 x, and what is lost of a small singular value there
+// is enlarged by every later step (final error on a 1024 x 1024 gradient: 4.2e-7 carried to the end, 5.2e-7 so, 7.8e-7 never;
+// fp32 products give 1.3e-6).
 //
 // a and a a are symmetric: only tiles on and above the diagonal are computed and written twice.
 //
@@ -132,7 +132,9 @@ struct PairGemm {
     const _Float16* p;        // rows i
     const _Float16* q;        // rows j
     const _Float16* a;        // POLYNOMIAL: a itself
-    float* carried;           // APPLY, FINISH
+    float* carried;           // APPLY, FINISH: x in fp32
+    const _Float16* was_t;    // and the pairs of its transpose
+    bool from_carried, to_carried;
     _Float16* out;            // GRAM, POLYNOMIAL: the symmetric result; APPLY: x
     _Float16* out_t;          // APPLY: its transpose
     void* result;             // FINISH
@@ -146,7 +148,7 @@ struct PairGemm {
     size_t p_stride, q_stride, a_stride, out_stride, result_stride;   // from one matrix of the batch to the next
     float unscale;            // of the accumulated product
     float c0, c1, c2;
-    float a_unscale, up;      // of a's parts; 2^e of the result
+    float a_unscale, up;      // of the parts of a or of x; 2^e of the result
 };
 
 // Tile number -> (ti, tj): all of them, ti fastest (workgroups that run together share columns of x),
@@ -165,6 +167,15 @@ __device__ __forceinline__ void tile_of(int id, int tiles_i, int& ti, int& tj)
     }
 }
 
+// a of the lanes where `upper` is not set and b of the lanes where it is, exchanged for the partner's other one
+template <int PARTNER>
+__device__ __forceinline__ void swap_across(unsigned& a, unsigned& b, bool upper)
+{
+    const unsigned got = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(upper ? a : b), PARTNER, 0xF, 0xF, true);
+    a = upper ? got : a;
+    b = upper ? b : got;
+}
+
 // What becomes of one block of 16 x 16 sums: a lane holds column lane & 15 in four consecutive rows.
 template <int MODE>
 __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, int bj, bool mirror, floatx4 v, int lane)
@@ -175,10 +186,18 @@ __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, i
     const size_t turned = pair_at(c, row, g.jb);   // (column, rows): 4 consecutive halves
     if (MODE >= APPLY) {
         floatx4* x = reinterpret_cast<floatx4*>(g.carried + z * (g.out_stride / 2) + carried_at(bi, bj, g.ib) + lane * 4);
-        const floatx4 was = *x;
+        floatx4 was;
+        if (g.from_carried) {
+            was = *x;
+        } else {
+            const _Float16* t = g.was_t + z * g.out_stride + turned;
+            const f16x4 h = *reinterpret_cast<const f16x4*>(t), l = *reinterpret_cast<const f16x4*>(t + BLOCK);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) was[r] = ((float)h[r] + (float)l[r]) * g.a_unscale;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(g.c0, was[r], v[r]);
-        if (MODE == APPLY) *x = v;
+        if (MODE == APPLY && g.to_carried) *x = v;
     }
     if (MODE == FINISH) {
         const size_t base = z * g.result_stride;
@@ -208,14 +227,29 @@ __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, i
     _Float16* to = (MODE == APPLY ? g.out_t + z * g.out_stride : out) + turned;
     *reinterpret_cast<f16x4*>(to) = hi;
     *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
-    // and in the other order: x itself, or the mirrored tile of a symmetric result
+    // and in the other order: x itself, or the mirrored tile of a symmetric result.  Four rows of a
+    // column to four columns of a row: a 4 x 4 transposition among four lanes in a row, hi and lo in one
+    // word, so that the stores are 8 bytes a lane and whole lines a wave here too.
     if (MODE == APPLY || mirror) {
+        unsigned w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            _Float16* also = out + pair_at(row + r, c, g.ib);
-            also[0] = hi[r];
-            also[BLOCK] = lo[r];
+            const f16x2 both = {hi[r], lo[r]};
+            w[r] = __builtin_bit_cast(unsigned, both);
         }
+        swap_across<0xB1>(w[0], w[1], lane & 1);   // lane ^ 1
+        swap_across<0xB1>(w[2], w[3], lane & 1);
+        swap_across<0x4E>(w[0], w[2], lane & 2);   // lane ^ 2
+        swap_across<0x4E>(w[1], w[3], lane & 2);
+        uintx2 h, l;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            h[r] = (w[2 * r] & 0xFFFFu) | w[2 * r + 1] << 16;
+            l[r] = w[2 * r] >> 16 | (w[2 * r + 1] & 0xFFFF0000u);
+        }
+        _Float16* also = out + pair_at(row + (lane & 3), c & ~3, g.ib);
+        *reinterpret_cast<uintx2*>(also) = h;
+        *reinterpret_cast<uintx2*>(also + BLOCK) = l;
     }
 }
 
@@ -525,6 +559,11 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
         k.p = b;
         k.q = xt[s & 1];
         k.carried = carried;
+        k.was_t = xt[s & 1];
+        // what an error in x grows to depends on the steps that follow: x in 32 bits while four or more do
+        k.from_carried = steps - s >= 4;
+        k.to_carried = steps - s >= 5;
+        k.a_unscale = 1.f / up_x;
         k.out = x;
         k.out_t = xt[(s & 1) ^ 1];
         k.result = out;
