@@ -2310,7 +2310,7 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
     Timer timer(stream, seconds);
     if ((st = timer.start())) return st;
     st = timer.family(M <= 64 ? 2 : 0, [&] {
-        return launch_linear_q4(xo.dev, qo.dev, bias ? bo.dev : nullptr, yo.dev, type, M, lay, with_zeros != 0, ws, cur().model.cus, stream);
+        return launch_linear_q4(xo.dev, qo.dev, bias ? bo.dev : nullptr, yo.dev, type, M, lay, with_zeros != 0, ws, stream);
     });
     if (st) return st;
     if ((st = timer.stop())) return st;

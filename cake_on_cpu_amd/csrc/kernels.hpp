@@ -284,8 +284,12 @@ hipError_t launch_q4_dequantize(const void* q, void* w, int w_type, const Q4Layo
 hipError_t launch_q4_pack(const unsigned char* codes, const void* scales, const void* zeros, void* q, const Q4Layout& lay,
                           hipStream_t stream);
 hipError_t launch_linear_q4(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
-                            bool with_zeros, void* workspace, int cus, hipStream_t stream);
+                            bool with_zeros, void* workspace, hipStream_t stream);
 size_t linear_q4_workspace(int M, int N, int K, int type);
+// its part for many rows of x (q4_linear_bands.hip)
+size_t linear_q4_bands_workspace(int M, int N, int K, int type);
+hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
+                                  bool with_zeros, void* workspace, bool vec, hipStream_t stream);
 
 // Newton-Schulz iterations (orthogonalize.hip).  The layout's offsets are bytes into the workspace.
 struct OrthogonalizeLayout {
