@@ -44,8 +44,17 @@ def _stream(*arrays) -> int:
     for a in arrays:
         if _is_torch(a) and a.is_cuda:
             import torch
-            return torch.cuda.current_stream(a.device).cuda_stream
+            return _torch_stream(torch, a.device)
     return 0
+
+
+def _torch_stream(torch, device) -> int:
+    """The handle of torch's current stream on `device`, without the stream object where this torch
+    has the short way (0.1 us instead of 1.7: a short kernel's call is bound by the host)."""
+    short = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if short is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return short(device.index)
 
 
 def _numel(a) -> int:
@@ -508,10 +517,13 @@ _TYPE_CODES = {"float32": _lib.F32, "float16": _lib.F16, "bfloat16": _lib.BF16}
 
 def element_type(dtype) -> int:
     """CAKE_HIP_F32 / F16 / BF16 of a torch or numpy dtype or its name."""
-    name = dtype if isinstance(dtype, str) else str(dtype).replace("torch.", "") if not isinstance(dtype, type) else np.dtype(dtype).name
-    if name not in _TYPE_CODES:
-        raise TypeError(f"element type {dtype}: float32, float16 or bfloat16 needed")
-    return _TYPE_CODES[name]
+    code = _TYPE_CODES.get(dtype)
+    if code is None:
+        name = np.dtype(dtype).name if isinstance(dtype, (type, np.dtype)) else str(dtype).replace("torch.", "")
+        if name not in _TYPE_CODES:
+            raise TypeError(f"element type {dtype}: float32, float16 or bfloat16 needed")
+        code = _TYPE_CODES[dtype] = _TYPE_CODES[name]
+    return code
 
 
 def _any_ptr(a, what: str, of: int | None = None) -> int:

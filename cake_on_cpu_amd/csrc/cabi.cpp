@@ -2166,12 +2166,10 @@ static int workspace_of(void* given, size_t bytes, size_t align, DeviceBuffer& b
         return CAKE_HIP_OK;
     }
     if ((uintptr_t)given % align) return fail(CAKE_HIP_ERR_ARG, "workspace is not %zu-byte aligned", align);
-    if (bytes) {
-        hipPointerAttribute_t attr;
-        if (hipPointerGetAttributes(&attr, given) != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != cur().device) {
-            (void)hipGetLastError();
-            return fail(CAKE_HIP_ERR_ARG, "workspace must be memory of device %d", cur().device);
-        }
+    hipPointerAttribute_t attr;
+    if (hipPointerGetAttributes(&attr, given) != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != cur().device) {
+        (void)hipGetLastError();
+        return fail(CAKE_HIP_ERR_ARG, "workspace must be memory of device %d", cur().device);
     }
     *out = given;
     return CAKE_HIP_OK;

@@ -289,7 +289,7 @@ size_t linear_q4_workspace(int M, int N, int K, int type);
 // its part for many rows of x (q4_linear_bands.hip)
 size_t linear_q4_bands_workspace(int M, int N, int K, int type);
 hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
-                                  bool with_zeros, void* workspace, bool vec, hipStream_t stream);
+                                  bool with_zeros, void* workspace, hipStream_t stream);
 
 // Newton-Schulz iterations (orthogonalize.hip).  The layout's offsets are bytes into the workspace.
 struct OrthogonalizeLayout {

@@ -176,6 +176,52 @@ __device__ __forceinline__ void swap_across(unsigned& a, unsigned& b, bool upper
     b = upper ? b : got;
 }
 
+// Four values of one column (rows 4 (lane >> 4) + 0..3, column lane & 15 of block bi, bj) as pairs at
+// [column][rows]: 8 bytes a lane and whole lines a wave.
+__device__ __forceinline__ void store_along(_Float16* out, int bi, int bj, int row_blocks, f16x4 hi, f16x4 lo, int lane)
+{
+    _Float16* to = out + pair_at(bj * 16 + (lane & 15), bi * 16 + (lane >> 4) * 4, row_blocks);
+    *reinterpret_cast<f16x4*>(to) = hi;
+    *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
+}
+
+// The same values at [row][columns]: four rows of a column to four columns of a row is a 4 x 4
+// transposition among four lanes in a row, hi and lo in one word, so that the stores are 8 bytes a lane
+// here too.
+__device__ __forceinline__ void store_across(_Float16* out, int bi, int bj, int row_blocks, f16x4 hi, f16x4 lo, int lane)
+{
+    unsigned w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const f16x2 both = {hi[r], lo[r]};
+        w[r] = __builtin_bit_cast(unsigned, both);
+    }
+    swap_across<0xB1>(w[0], w[1], lane & 1);   // lane ^ 1
+    swap_across<0xB1>(w[2], w[3], lane & 1);
+    swap_across<0x4E>(w[0], w[2], lane & 2);   // lane ^ 2
+    swap_across<0x4E>(w[1], w[3], lane & 2);
+    uintx2 h, l;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        h[r] = (w[2 * r] & 0xFFFFu) | w[2 * r + 1] << 16;
+        l[r] = w[2 * r] >> 16 | (w[2 * r + 1] & 0xFFFF0000u);
+    }
+    _Float16* to = out + pair_at(bi * 16 + (lane >> 4) * 4 + (lane & 3), bj * 16 + (lane & 12), row_blocks);
+    *reinterpret_cast<uintx2*>(to) = h;
+    *reinterpret_cast<uintx2*>(to + BLOCK) = l;
+}
+
+__device__ __forceinline__ void split4(floatx4 v, float up, f16x4& hi, f16x4& lo)
+{
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        _Float16 h, l;
+        split(v[r] * up, h, l);
+        hi[r] = h;
+        lo[r] = l;
+    }
+}
+
 // What becomes of one block of 16 x 16 sums: a lane holds column lane & 15 in four consecutive rows.
 template <int MODE>
 __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, int bj, bool mirror, floatx4 v, int lane)
@@ -216,41 +262,11 @@ __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, i
         for (int r = 0; r < 4; ++r) v[r] = g.c2 * v[r] + g.c1 * (((float)ah[r] + (float)al[r]) * g.a_unscale);
     }
     f16x4 hi, lo;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        _Float16 h, l;
-        split(v[r] * g.up, h, l);
-        hi[r] = h;
-        lo[r] = l;
-    }
+    split4(v, g.up, hi, lo);
     _Float16* out = g.out + z * g.out_stride;
-    _Float16* to = (MODE == APPLY ? g.out_t + z * g.out_stride : out) + turned;
-    *reinterpret_cast<f16x4*>(to) = hi;
-    *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
-    // and in the other order: x itself, or the mirrored tile of a symmetric result.  Four rows of a
-    // column to four columns of a row: a 4 x 4 transposition among four lanes in a row, hi and lo in one
-    // word, so that the stores are 8 bytes a lane and whole lines a wave here too.
-    if (MODE == APPLY || mirror) {
-        unsigned w[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const f16x2 both = {hi[r], lo[r]};
-            w[r] = __builtin_bit_cast(unsigned, both);
-        }
-        swap_across<0xB1>(w[0], w[1], lane & 1);   // lane ^ 1
-        swap_across<0xB1>(w[2], w[3], lane & 1);
-        swap_across<0x4E>(w[0], w[2], lane & 2);   // lane ^ 2
-        swap_across<0x4E>(w[1], w[3], lane & 2);
-        uintx2 h, l;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            h[r] = (w[2 * r] & 0xFFFFu) | w[2 * r + 1] << 16;
-            l[r] = w[2 * r] >> 16 | (w[2 * r + 1] & 0xFFFF0000u);
-        }
-        _Float16* also = out + pair_at(row + (lane & 3), c & ~3, g.ib);
-        *reinterpret_cast<uintx2*>(also) = h;
-        *reinterpret_cast<uintx2*>(also + BLOCK) = l;
-    }
+    store_along(MODE == APPLY ? g.out_t + z * g.out_stride : out, bi, bj, g.jb, hi, lo, lane);
+    // and in the other order: x itself, or the mirrored tile of a symmetric result
+    if (MODE == APPLY || mirror) store_across(out, bi, bj, g.ib, hi, lo, lane);
 }
 
 // out = P . Q^T over WI x WJ waves of TI x TJ blocks of 16 x 16 each.  A stage is one column block (32
@@ -484,6 +500,167 @@ size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
     return (size_t)tile_count(blocks, ib, jb, symmetric) * t.slices * batch * blocks * blocks * 256;
 }
 
+// ---- small matrices ------------------------------------------------------------------------
+// One workgroup per matrix and one launch: a matrix whose pairs and whose square's pairs fit the LDS of a
+// compute unit together (sides up to 128 x 160, 64 x 560, 32 x 1200).  x stays in registers in fp32, in
+// blocks as they come out of the matrix pipe; its pairs are written to LDS along its columns for
+// a = x x^T and then, over them, along its rows for b x.  Launches of a product each cost 5 to 6 us
+// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, SMALLUS in one.
+enum { SMALL_WAVES = 16, SMALL_X_BLOCKS = 10, SMALL_A_BLOCKS = 3 };   // blocks a wave holds of x and of the square
+
+struct SmallArgs {
+    const void* g;
+    void* out;
+    int type, m, n, mb, nb, steps;
+    bool tall;
+    float c0, c1, c2;
+    double eps;
+    float up_x, up_a, up_b;
+};
+
+__device__ __forceinline__ floatx4 pair_product(const _Float16* p, const _Float16* q, int step_p, int step_q, int kb)
+{
+    floatx4 acc = {0, 0, 0, 0};
+    for (int k = 0; k < kb; ++k) {
+        const f16x8 ph = *reinterpret_cast<const f16x8*>(p), pl = *reinterpret_cast<const f16x8*>(p + BLOCK);
+        const f16x8 qh = *reinterpret_cast<const f16x8*>(q), ql = *reinterpret_cast<const f16x8*>(q + BLOCK);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+        p += step_p;
+        q += step_q;
+    }
+    return acc;
+}
+
+__global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallArgs s)
+{
+    extern __shared__ __align__(16) _Float16 stage[];
+    __shared__ double norms[SMALL_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    _Float16* const xs = stage;                          // pairs of x, then of its transpose
+    _Float16* const as = stage + s.mb * s.nb * BLOCK;    // pairs of a, then of b
+    const int blocks = s.mb * s.nb, squares = s.mb * (s.mb + 1) / 2;
+    const size_t base = (size_t)blockIdx.x * s.m * s.n;
+    auto index = [&](int i, int j) { return base + (s.tall ? (size_t)j * s.m + i : (size_t)i * s.n + j); };
+
+    floatx4 x[SMALL_X_BLOCKS];
+    double sum = 0;
+#pragma unroll
+    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
+        const int block = wave + t * waves;
+        x[t] = floatx4{0, 0, 0, 0};
+        if (block < blocks) {
+            const int i = block % s.mb * 16 + (lane >> 4) * 4, j = block / s.mb * 16 + (lane & 15);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (i + r < s.m && j < s.n) {
+                    x[t][r] = load_as_float(s.g, index(i + r, j), s.type);
+                    sum += (double)x[t][r] * (double)x[t][r];
+                }
+        }
+    }
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) norms[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < waves; ++w) sum += norms[w];
+    const double length = sqrt(sum) + s.eps;
+    const double by = length == 0 ? 0 : 1.0 / length;   // zeros stay zeros also without an eps
+#pragma unroll
+    for (int t = 0; t < SMALL_X_BLOCKS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t][r] = (float)((double)x[t][r] * by);
+
+    const float down_aa = 1.f / (s.up_a * s.up_a), down_xx = 1.f / (s.up_x * s.up_x), down_bx = 1.f / (s.up_b * s.up_x), down_a = 1.f / s.up_a;
+    auto store_x = [&](bool along) {
+#pragma unroll
+        for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
+            const int block = wave + t * waves;
+            if (block < blocks) {
+                f16x4 hi, lo;
+                split4(x[t], s.up_x, hi, lo);
+                if (along) store_along(xs, block % s.mb, block / s.mb, s.nb, hi, lo, lane);
+                else store_across(xs, block % s.mb, block / s.mb, s.mb, hi, lo, lane);
+            }
+        }
+    };
+    for (int step = 0; step < s.steps; ++step) {
+        store_x(false);
+        __syncthreads();
+        floatx4 square[SMALL_A_BLOCKS];
+        auto store_squares = [&](float up) {
+#pragma unroll
+            for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
+                int bi, bj;
+                tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+                if (wave + t * waves < squares) {
+                    f16x4 hi, lo;
+                    split4(square[t], up, hi, lo);
+                    store_along(as, bi, bj, s.mb, hi, lo, lane);
+                    if (bi != bj) store_across(as, bi, bj, s.mb, hi, lo, lane);
+                }
+            }
+        };
+        const int step_a = s.mb * 2 * BLOCK;
+#pragma unroll
+        for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
+            int bi, bj;
+            tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+            if (wave + t * waves < squares) {
+                const floatx4 v = pair_product(xs + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.nb / 2);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) square[t][r] = v[r] * down_xx;
+            }
+        }
+        store_squares(s.up_a);   // the first time into memory that nobody reads, then behind the barrier after b x
+        __syncthreads();
+        store_x(true);           // a is complete: nobody reads x along its columns any more
+#pragma unroll
+        for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
+            int bi, bj;
+            tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+            if (wave + t * waves < squares) {
+                const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, as + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.mb / 2);
+                const _Float16* a = as + pair_at(bj * 16 + (lane & 15), bi * 16 + (lane >> 4) * 4, s.mb);
+                const f16x4 ah = *reinterpret_cast<const f16x4*>(a), al = *reinterpret_cast<const f16x4*>(a + BLOCK);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) square[t][r] = s.c2 * (v[r] * down_aa) + s.c1 * (((float)ah[r] + (float)al[r]) * down_a);
+            }
+        }
+        __syncthreads();
+        store_squares(s.up_b);
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
+            const int block = wave + t * waves;
+            if (block < blocks) {
+                const int bi = block % s.mb, bj = block / s.mb;
+                const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, s.nb * 2 * BLOCK, s.mb / 2);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[t][r] = __builtin_fmaf(s.c0, x[t][r], v[r] * down_bx);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
+        const int block = wave + t * waves;
+        if (block < blocks) {
+            const int i = block % s.mb * 16 + (lane >> 4) * 4, j = block / s.mb * 16 + (lane & 15);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (i + r < s.m && j < s.n) store_from_float(s.out, index(i + r, j), s.type, x[t][r]);
+        }
+    }
+}
+
+// a block of 16 x 32 pairs is 2 KB: mb nb / 2 of them for x, mb mb / 2 for the square, 1 KB left for the norm
+bool small_fits(int mb, int nb)
+{
+    return mb * nb + mb * mb <= 159 && mb * nb <= SMALL_WAVES * SMALL_X_BLOCKS && mb * (mb + 1) / 2 <= SMALL_WAVES * SMALL_A_BLOCKS;
+}
+
 }  // namespace
 
 OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols)
@@ -505,7 +682,7 @@ OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols)
     l.slices = l.carried + (size_t)batch * l.x_halves * 2;
     const size_t floats[3] = {slice_floats(l.mb, l.mb, l.nb / 2, true, batch), slice_floats(l.mb, l.mb, l.mb / 2, true, batch),
                               slice_floats(l.mb, l.nb, l.mb / 2, false, batch)};
-    l.bytes = l.slices + std::max(floats[0], std::max(floats[1], floats[2])) * sizeof(float);
+    l.bytes = small_fits(l.mb, l.nb) ? 0 : l.slices + std::max(floats[0], std::max(floats[1], floats[2])) * sizeof(float);
     return l;
 }
 
@@ -513,6 +690,20 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
                                 double c2, double eps, const OrthogonalizeScales& sc, void* workspace, hipStream_t stream)
 {
     const OrthogonalizeLayout l = orthogonalize_layout(batch, rows, cols);
+    const float up_x = ldexpf(1.f, sc.ex), up_a = ldexpf(1.f, sc.ea), up_b = ldexpf(1.f, sc.eb);
+    const bool tall = rows > cols;
+    if (small_fits(l.mb, l.nb)) {
+        SmallArgs a{g, out, type, l.m, l.n, l.mb, l.nb, steps, tall, (float)c0, (float)c1, (float)c2, eps, up_x, up_a, up_b};
+        const size_t lds = (size_t)(l.mb * l.nb + l.mb * l.mb) * 1024;
+        if (lds > 63 * 1024) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&small_matrices_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        // a wave per block of x at least while there are more waves than that; squares never need more than the same
+        const int waves = std::min<int>(SMALL_WAVES, l.mb * l.nb);
+        small_matrices_kernel<<<batch, 64 * waves, lds, stream>>>(a);
+        return hipGetLastError();
+    }
     char* ws = static_cast<char*>(workspace);
     _Float16* x = reinterpret_cast<_Float16*>(ws + l.x);
     _Float16* xt[2] = {reinterpret_cast<_Float16*>(ws + l.xt0), reinterpret_cast<_Float16*>(ws + l.xt1)};
@@ -522,13 +713,11 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     float* carried = reinterpret_cast<float*>(ws + l.carried);
     float* slices = reinterpret_cast<float*>(ws + l.slices);
     const size_t values = (size_t)l.m * l.n;
-    const bool tall = rows > cols;
     const size_t want = (values + 8191) / 8192;
     const int chunks = want < NORM_CHUNKS ? (int)want : NORM_CHUNKS;
     norm_partial_kernel<<<dim3(chunks, batch), 256, 0, stream>>>(g, type, partial, values);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const float up_x = ldexpf(1.f, sc.ex), up_a = ldexpf(1.f, sc.ea), up_b = ldexpf(1.f, sc.eb);
     normalize_kernel<<<dim3((l.nb + 3) / 4, (l.mb + 3) / 4, batch), 256, 0, stream>>>(g, type, partial, chunks, eps, up_x, x, xt[0], carried, l.m,
                                                                                      l.n, l.mb, l.nb, tall, l.x_halves);
     if ((e = hipGetLastError()) != hipSuccess) return e;

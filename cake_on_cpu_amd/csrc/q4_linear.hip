@@ -39,15 +39,90 @@ struct StreamArgs {
     void* y;
     Q4Layout lay;
     int M, with_zeros;
-    int chunk_blocks;     // blocks of 128 columns of x held in LDS at a time, a multiple of the waves
-    int zero_at;          // byte offset in LDS of 16 zero bytes, behind the chunk
-    bool vec;
 };
 
-// Few rows of x (up to 16 of pieces): the codes are read once, straight into the registers of the wave that
-// multiplies them, x lies in LDS as the matrix pipe's A operand.  A workgroup owns NT tiles of 16
-// rows of v; its waves share the blocks of 128 columns out among them in turn, DEPTH turns in
-// flight each, and add their sums up through LDS in a fixed order.
+// x of one block of 128 columns on its way to the matrix pipe's A operand.  16-bit x: every lane fetches
+// its 8 columns of its row for each of the four steps, straight in operand order.  32-bit x: the wave
+// fetches two columns a lane, cuts them into pieces and passes them through LDS of its own; no
+// other wave takes part, so nothing waits at a barrier.
+template <int TYPE, int REGS>
+struct BlockOfX {
+    typedef typename Element<TYPE>::T T;
+    uintx4 step[4];
+    __device__ __forceinline__ void fetch(const T* x, int M, int K, int block, int lane, int my_row)
+    {
+        const int k = block * 128 + (lane >> 4) * 8;
+        const bool whole = block * 128 + 128 <= K;   // the same for the whole wave
+#pragma unroll
+        for (int i = 0; i < 4; ++i) step[i] = uintx4{0, 0, 0, 0};
+        if (my_row < M) {
+            const T* at = x + (size_t)my_row * K + k;
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) __builtin_memcpy(&step[i], at + 32 * i, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    T v[8];
+                    load_eight<TYPE>(at + 32 * i, K - k - 32 * i, v);
+                    step[i] = piece_of<TYPE>(v, 0);
+                }
+            }
+        }
+    }
+    static constexpr int TOKENS = 0;
+    __device__ __forceinline__ void to_lds(unsigned char*, int) const {}
+    __device__ __forceinline__ uintx4 operand(int i, const unsigned char*, bool) const { return step[i]; }
+};
+template <int REGS>
+struct BlockOfX<CAKE_HIP_F32, REGS> {
+    static constexpr int TOKENS = REGS == 1 ? 1 : 5;   // whose pieces fill 4 or 16 rows
+    float v[TOKENS][2];
+    __device__ __forceinline__ void fetch(const float* x, int M, int K, int block, int lane, int)
+    {
+        const int k = block * 128 + lane * 2;
+        const bool whole = block * 128 + 128 <= K;
+#pragma unroll
+        for (int m = 0; m < TOKENS; ++m) {
+            const float* at = x + (size_t)(m < M ? m : 0) * K + k;
+            if (whole) {
+                __builtin_memcpy(v[m], at, 8);
+            } else {
+                v[m][0] = k < K ? at[0] : 0.f;
+                v[m][1] = k + 1 < K ? at[1] : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void to_lds(unsigned char* mine, int lane) const
+    {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last block has been read
+#pragma unroll
+        for (int m = 0; m < TOKENS; ++m) {
+            float rest[2] = {v[m][0], v[m][1]};
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                unsigned cut[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    cut[j] = __builtin_bit_cast(unsigned, rest[j]) & 0xFFFF0000u;
+                    rest[j] -= __builtin_bit_cast(float, cut[j]);   // exact
+                }
+                *reinterpret_cast<unsigned*>(mine + ((lane >> 4) * TOKENS * 3 + m * 3 + p) * 64 + (lane & 15) * 4) = cut[0] >> 16 | cut[1];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __device__ __forceinline__ uintx4 operand(int i, const unsigned char* mine_row, bool real) const
+    {
+        const uintx4 got = *reinterpret_cast<const uintx4*>(mine_row + i * TOKENS * 3 * 64);
+        return real ? got : uintx4{0, 0, 0, 0};
+    }
+};
+
+// Few rows of x (up to 16 of pieces): the codes are read once, straight into the registers of the
+// wave that multiplies them.  A workgroup owns NT tiles of 16 rows of v; its waves share the blocks of
+// 128 columns out among them in turn, DEPTH turns in flight each, and add their sums up through LDS
+// in a fixed order.
 // Row r of pieces is A's row 4 (r & 3) + (r >> 2), so that the first four rows come out in the four lanes'
 // first result register and REGS registers cover 4 REGS rows: with one token the scale costs two
 // operations per group instead of eight.
@@ -65,15 +140,17 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
     const int rows = a.M * PIECES;
     const int tile0 = blockIdx.x * NT;
 
-    // this lane's row of the A operand, or the zeros
+    // this lane's row of the A operand, and the place of its columns in the wave's own LDS (32-bit x)
     const int my_row = (col & 3) * 4 + (col >> 2);
-    const unsigned a_base = my_row < rows ? my_row * 64 + quad * 16 : a.zero_at;
-    const unsigned a_step = my_row < rows ? rows * 64 : 0;
-    if (threadIdx.x < 4) reinterpret_cast<unsigned*>(lds + a.zero_at)[threadIdx.x] = 0;
+    const bool real = my_row < rows;
+    constexpr int OWN = BlockOfX<TYPE, REGS>::TOKENS * 3 * 256;
+    unsigned char* mine = lds + wave * OWN;
+    const unsigned char* mine_row = mine + (real ? my_row * 64 + quad * 16 : 0);
 
     struct Held {
         uintx4 code[NT];
         GroupValues<GPB, WIDE> s[NT], z[NT];
+        BlockOfX<TYPE, REGS> x;
     } held[DEPTH];
     // addresses are scalars that move on by the waves' number of blocks, and a lane's place in a block
     constexpr int SCALE_BYTES = 16 * GPB * (WIDE ? 4 : 2);
@@ -98,6 +175,7 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
                 scale_at[nt] += waves * SCALE_BYTES;
                 zero_at[nt] += waves * SCALE_BYTES;
             }
+            h.x.fetch(static_cast<const T*>(a.x), a.M, K, fetched, lane, my_row);
         }
         fetched += waves;
     };
@@ -109,7 +187,8 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) ones[i] = Codes<TYPE>::ONES;
 
-    auto multiply = [&](const Held& h, int step0) {
+    auto multiply = [&](const Held& h) {
+        h.x.to_lds(mine, lane);
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
             floatx4 p[NT], sum = floatx4{0, 0, 0, 0};
@@ -117,7 +196,7 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
             for (int nt = 0; nt < NT; ++nt) p[nt] = floatx4{0, 0, 0, 0};
 #pragma unroll
             for (int i = g * SG; i < (g + 1) * SG; ++i) {
-                const uintx4 xa = *reinterpret_cast<const uintx4*>(lds + a_base + a_step * (unsigned)(step0 + i));
+                const uintx4 xa = h.x.operand(i, mine_row, real);
                 sum = Codes<TYPE>::mfma(xa, ones, sum);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) p[nt] = Codes<TYPE>::mfma(xa, unpack_codes<TYPE>(h.code[nt][i]), p[nt]);
@@ -131,36 +210,16 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
         }
     };
 
-    const int turns = (blocks + waves - 1) / waves, turns_per_chunk = a.chunk_blocks / waves;
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) fetch(held[d]);
-    int block = wave, chunk0 = 0, until_chunk = 0;
-    for (int t0 = 0; t0 < turns; t0 += DEPTH) {
+    for (int block = wave; block < blocks;) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            if (t0 + d < turns) {   // the same for every wave of the workgroup
-                if (until_chunk == 0) {
-                    chunk0 = (t0 + d) * waves;
-                    until_chunk = turns_per_chunk;
-                    if (chunk0) __syncthreads();
-                    // the next chunk of x: piece p of row m at [step of 32 columns][m * PIECES + p][8-column part]
-                    const int parts = min(a.chunk_blocks, blocks - chunk0) * 16;
-                    for (int m = 0; m < a.M; ++m)
-                        for (int part = threadIdx.x; part < parts; part += blockDim.x) {
-                            const int k = chunk0 * 128 + part * 8;
-                            T v[8];
-                            load_eight<TYPE>(static_cast<const T*>(a.x) + (size_t)m * K + k, K - k, a.vec, v);
-#pragma unroll
-                            for (int p = 0; p < PIECES; ++p)
-                                *reinterpret_cast<uintx4*>(lds + ((part >> 2) * rows + m * PIECES + p) * 64 + (part & 3) * 16) = piece_of<TYPE>(v, p);
-                        }
-                    __syncthreads();
-                }
-                --until_chunk;
-                if (block < blocks) multiply(held[d], (block - chunk0) * 4);
+            if (block < blocks) {
+                multiply(held[d]);
                 fetch(held[d]);
-                block += waves;
             }
+            block += waves;
         }
     }
 
@@ -189,26 +248,18 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
 }
 
 template <int TYPE, int GPB>
-hipError_t stream_launch(StreamArgs a, hipStream_t stream)
+hipError_t stream_launch(const StreamArgs& a, hipStream_t stream)
 {
     const int rows = a.M * pieces_of<TYPE>();
     // two tiles a workgroup share x and its column sums, as soon as that leaves a workgroup for every compute unit
     const int nt = a.lay.tiles >= 512 ? 2 : 1;
     int waves = nt == 1 ? 16 : 8;
     while (waves > 1 && waves / 2 >= a.lay.blocks) waves /= 2;
-    // a chunk of x of at most 32 KB (one turn of the waves at least)
-    const int block_bytes = rows * 256;
-    const int all_turns = (a.lay.blocks + waves - 1) / waves;
-    const int turns = std::max(1, std::min(all_turns, 32 * 1024 / (block_bytes * waves)));
-    a.chunk_blocks = turns * waves;
-    a.zero_at = a.chunk_blocks * block_bytes;
-    const size_t lds = std::max((size_t)waves * rows * nt * 16 * 4, (size_t)a.zero_at + 16);
+    // the waves' sums; before that, of a 32-bit x, their blocks of pieces
+    const size_t own = TYPE == CAKE_HIP_F32 ? (rows <= 4 ? 3 : 15) * 256 : 0;
+    const size_t lds = waves * std::max((size_t)rows * nt * 64, own);
     const dim3 grid((a.lay.tiles + nt - 1) / nt), block(64 * waves);
     auto run = [&](auto kernel) {
-        if (lds > 64 * 1024) {
-            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (e != hipSuccess) return e;
-        }
         kernel<<<grid, block, lds, stream>>>(a);
         return hipGetLastError();
     };
@@ -220,22 +271,21 @@ hipError_t stream_launch(StreamArgs a, hipStream_t stream)
     return a.lay.scale_type == CAKE_HIP_F32 ? of_width(std::true_type()) : of_width(std::false_type());
 }
 
-// One tile of 16 rows of pieces is streamed; K == 0 is only a bias, which the streaming kernel writes for any M
-bool streams(int M, int K, int type) { return K == 0 || M <= (type == CAKE_HIP_F32 ? 5 : 16); }
+// what fits one tile of 16 rows of pieces is streamed
+bool streams(int M, int type) { return M <= (type == CAKE_HIP_F32 ? 5 : 16); }
 
 }  // namespace
 
 size_t linear_q4_workspace(int M, int N, int K, int type)
 {
-    return M == 0 || N == 0 || streams(M, K, type) ? 0 : linear_q4_bands_workspace(M, N, K, type);
+    return M == 0 || N == 0 || streams(M, type) ? 0 : linear_q4_bands_workspace(M, N, K, type);
 }
 
 hipError_t launch_linear_q4(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
                             bool with_zeros, void* workspace, hipStream_t stream)
 {
-    const bool vec = lay.K % 8 == 0 && (uintptr_t)x % 16 == 0;
     hipError_t e = hipSuccess;
-    if (streams(M, lay.K, type)) {
+    if (streams(M, type)) {
         StreamArgs a{};
         a.x = x;
         a.q = static_cast<const unsigned char*>(q);
@@ -244,12 +294,11 @@ hipError_t launch_linear_q4(const void* x, const void* q, const void* bias, void
         a.lay = lay;
         a.M = M;
         a.with_zeros = with_zeros;
-        a.vec = vec;
         q4_for_type_and_group(type, lay.groups_per_block,
                               [&](auto t, auto gpb) { e = stream_launch<decltype(t)::value, decltype(gpb)::value>(a, stream); });
         return e;
     }
-    return launch_linear_q4_bands(x, q, bias, y, type, M, lay, with_zeros, workspace, vec, stream);
+    return launch_linear_q4_bands(x, q, bias, y, type, M, lay, with_zeros, workspace, stream);
 }
 
 }  // namespace cake

@@ -34,7 +34,6 @@ struct BandArgs {
     float* partial;       // [slice][M][N], or nullptr
     Q4Layout lay;
     int M, bands, stages, slices;
-    bool vec;
 };
 
 // x into records: a wave per tile and stage.
@@ -56,7 +55,7 @@ __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
     for (int i = 0; i < R::STEPS; ++i) {
         const int k = (stage * R::STEPS + i) * 32 + (lane >> 4) * 8;
         T v[8];
-        load_eight<TYPE>(static_cast<const T*>(a.x) + (size_t)row * a.lay.K + k, row < a.M ? a.lay.K - k : 0, a.vec, v);
+        load_eight<TYPE>(static_cast<const T*>(a.x) + (size_t)row * a.lay.K + k, row < a.M ? a.lay.K - k : 0, v);
 #pragma unroll
         for (int p = 0; p < R::PIECES; ++p)
             *reinterpret_cast<uintx4*>(to + ((tile * R::STEPS + i) * R::PIECES + p) * 1024 + lane * 16) = piece_of<TYPE>(v, p);
@@ -297,9 +296,11 @@ hipError_t band_launch(const BandArgs& a, hipStream_t stream)
 {
     typedef Record<TYPE, GROUPS, MTW> R;
     const size_t units = (size_t)a.bands * a.stages * R::TILES;
-    linear_q4_records_kernel<TYPE, GROUPS, MTW, ZEROS><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e = hipSuccess;
+    if (units) {   // (K == 0 is only a bias)
+        linear_q4_records_kernel<TYPE, GROUPS, MTW, ZEROS><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     constexpr size_t LDS = (size_t)2 * R::KB * 1024;
     auto kernel = &linear_q4_band_kernel<TYPE, GROUPS, MTW, ZEROS>;
     if (LDS > 64 * 1024) {
@@ -327,7 +328,7 @@ hipError_t bands_launch(const BandArgs& a, int mtw, bool zeros, hipStream_t stre
 size_t linear_q4_bands_workspace(int M, int N, int K, int type) { return band_plan(M, N, K, type).bytes; }
 
 hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
-                                  bool with_zeros, void* workspace, bool vec, hipStream_t stream)
+                                  bool with_zeros, void* workspace, hipStream_t stream)
 {
     const BandPlan p = band_plan(M, lay.N, lay.K, type);
     BandArgs a{};
@@ -342,7 +343,6 @@ hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias
     a.bands = p.bands;
     a.stages = p.stages;
     a.slices = p.slices;
-    a.vec = vec;
     const bool two = type != CAKE_HIP_F32 && lay.groups_per_block == 4;
     if (type == CAKE_HIP_F32) return bands_launch<CAKE_HIP_F32, 1>(a, p.mtw, with_zeros, stream);
     if (type == CAKE_HIP_F16)

@@ -56,15 +56,14 @@ __device__ __forceinline__ uintx4 unpack_codes(unsigned word)
     return b;
 }
 
-// eight consecutive elements of a row of x, zero from column K on
+// Eight consecutive elements of a row of x, zero from `left` on.  Rows start at any element: the
+// hardware's 16-byte loads take any address.
 template <int TYPE>
-__device__ __forceinline__ void load_eight(const typename Element<TYPE>::T* at, int left, bool vec, typename Element<TYPE>::T (&v)[8])
+__device__ __forceinline__ void load_eight(const typename Element<TYPE>::T* at, int left, typename Element<TYPE>::T (&v)[8])
 {
     typedef typename Element<TYPE>::T T;
-    if (vec && left >= 8) {
-        struct alignas(16) Eight { T e[8]; } got = *reinterpret_cast<const Eight*>(at);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = got.e[e];
+    if (left >= 8) {
+        __builtin_memcpy(v, at, sizeof v);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = e < left ? at[e] : (T)0.f;

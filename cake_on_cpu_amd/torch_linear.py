@@ -136,12 +136,22 @@ def dequantize_q4(q, dtype=torch.float32):
 
 
 def _forward_q4(x, q, bias):
+    """x and bias contiguous, on the weights' device, checked by the caller"""
     M = x.size(0)
-    y = torch.empty((M, q.N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((M, q.N))
+    if not x.is_cuda:
+        api.linear_q4_forward(x, q, bias, y, M)
+        return y
+    # one token is a few microseconds of device time: straight into the C entry, which checks sizes, types and
+    # devices itself
+    t = api.element_type(x.dtype)
+    lib = api.load()
     # a workspace from torch's allocator belongs to this call's stream, and to a graph if one is captured
-    need = api.linear_q4_workspace(M, q.N, q.K, x.dtype) if x.is_cuda and M > 1 else 0
+    need = lib.cake_hip_linear_q4_workspace(M, q.N, q.K, t) if M > 1 else 0
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    api.linear_q4_forward(x, q, bias, y, M, workspace=ws, timed=not x.is_cuda)
+    api.check(lib.cake_hip_linear_q4_forward(x.data_ptr(), q.data.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), t,
+                                             M, q.N, q.K, q.group, q.scale_type, q.with_zeros, None if ws is None else ws.data_ptr(),
+                                             api._torch_stream(torch, x.device), None), "forward_q4")
     return y
 
 
@@ -169,6 +179,8 @@ def forward_q4(input, q, bias=None):
     float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias."""
     if input.dim() != 2 or input.size(1) != q.K:
         raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
+    if not q.data.is_contiguous():
+        raise TypeError("forward_q4: packed weights must be contiguous")
     if bias is not None and (tuple(bias.shape) != (q.N,) or bias.dtype != input.dtype):
         raise ValueError(f"forward_q4: bias {tuple(bias.shape)} of {bias.dtype} does not match {q.N} outputs of {input.dtype}")
     if input.device != q.data.device or (bias is not None and bias.device != input.device):

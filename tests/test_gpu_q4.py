@@ -127,6 +127,9 @@ def test_empty_dimensions_and_host_operands():
     assert np.array_equal(y, np.broadcast_to(bias, (3, 5)))
     cake.linear_q4_forward(np.zeros(1, f32), empty, None, y, 3)
     assert not y.any()
+    many = np.full((700, 5), np.nan, f32)                                # and for many rows
+    cake.linear_q4_forward(np.zeros(1, f32), empty, bias, many, 700)
+    assert np.array_equal(many, np.broadcast_to(bias, (700, 5)))
     N, K, M = 70, 333, 5
     packed, s, z, v64, mass = _weights(N, K, 32, True, torch.float32, 2)
     q = cake.q4_pack(packed.numpy(), s.numpy(), z.numpy(), N, K, 32)

@@ -82,7 +82,7 @@ def test_orthogonalize_workspace_covers_its_parts():
     ws = cake.orthogonalize_workspace
     assert ws(0, 4, 4) == 0 and ws(1, 0, 4) == 0 and ws(-1, 4, 4) == 0 and ws(1, 1 << 20, 1 << 20) == 0
     # at least three copies of x and two of the small square, each 4 bytes a padded value; the same on every call
-    for batch, rows, cols in ((1, 1, 1), (3, 33, 100), (2, 100, 33), (1, 1024, 4096)):
+    for batch, rows, cols in ((2, 300, 200), (2, 200, 300), (1, 1024, 4096)):
         m, n = (-(-v // 32) * 32 for v in sorted((rows, cols)))
         assert ws(batch, rows, cols) >= batch * (3 * m * n * 4 + 2 * m * m * 4) and ws(batch, rows, cols) == ws(batch, rows, cols)
 
