@@ -53,16 +53,25 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo)
     lo = (_Float16)(v - (float)hi);
 }
 
-// Sums of squares in 64 bits, so that no gradient is too small or too large for its norm.
-__global__ __launch_bounds__(256) void norm_partial_kernel(const void* __restrict__ g, int type, double* __restrict__ partial, size_t values)
+// Sums of squares in 64 bits, so that no gradient is too small or too large for its norm.  Eight values a
+// lane and load; the hardware takes them at any address.
+template <int TYPE>
+__global__ __launch_bounds__(256) void norm_partial_kernel(const typename Element<TYPE>::T* __restrict__ g, double* __restrict__ partial, size_t values)
 {
+    typedef typename Element<TYPE>::T T;
     __shared__ double red[4];
-    const size_t base = (size_t)blockIdx.y * values;
+    g += (size_t)blockIdx.y * values;
     double sum = 0;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < values; i += (size_t)gridDim.x * 256) {
-        const double v = (double)load_as_float(g, base + i, type);
-        sum += v * v;
+    const size_t step = (size_t)gridDim.x * 256 * 8;
+    size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    for (; i + 8 <= values; i += step) {
+        T v[8];
+        __builtin_memcpy(v, g + i, sizeof v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += (double)(float)v[e] * (double)(float)v[e];
     }
+    for (int e = 0; e < 8; ++e)   // the last, incomplete eight are one lane's
+        if (i + e < values) sum += (double)(float)g[i + e] * (double)(float)g[i + e];
     for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
     __syncthreads();
@@ -416,7 +425,7 @@ struct TileCost {
     int blocks, resident;
     float alone, full;
 };
-constexpr TileCost TILES[] = {{4, 4, 0.47f, 0.95f}, {8, 2, 0.75f, 1.35f}, {12, 1, 1.42f, 1.42f}, {16, 1, 2.3f, 2.3f}};
+constexpr TileCost TILES[] = {{4, 4, 0.42f, 1.1f}, {8, 2, 0.75f, 1.42f}, {12, 1, 1.42f, 1.42f}, {16, 1, 2.35f, 2.35f}};
 // The device's compute units; a number of this file, so that the size of the workspace and the order of
 // the sums follow from the sizes alone.
 constexpr int CUS = 256;
@@ -485,7 +494,7 @@ hipError_t pair_gemm(PairGemm g, int batch, float* partial, hipStream_t stream)
     g.partial = t.slices > 1 ? partial : nullptr;
     switch (t.which) {
     case 0: return pair_gemm_on<MODE, 2, 2, 2, 2>(g, batch, stream);
-    case 1: return pair_gemm_on<MODE, 2, 2, 4, 4>(g, batch, stream);
+    case 1: return pair_gemm_on<MODE, 2, 4, 4, 2>(g, batch, stream);
     case 2: return pair_gemm_on<MODE, 2, 4, 6, 3>(g, batch, stream);
     default: return pair_gemm_on<MODE, 2, 4, 8, 4>(g, batch, stream);
     }
@@ -505,7 +514,7 @@ size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
 // compute unit together (sides up to 128 x 160, 64 x 560, 32 x 1200).  x stays in registers in fp32, in
 // blocks as they come out of the matrix pipe; its pairs are written to LDS along its columns for
 // a = x x^T and then, over them, along its rows for b x.  Launches of a product each cost 5 to 6 us
-// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, SMALLUS in one.
+// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 49 us in one.
 enum { SMALL_WAVES = 16, SMALL_X_BLOCKS = 10, SMALL_A_BLOCKS = 3 };   // blocks a wave holds of x and of the square
 
 struct SmallArgs {
@@ -518,19 +527,31 @@ struct SmallArgs {
     float up_x, up_a, up_b;
 };
 
+// The sum over kb column blocks of one block's product.  The next operands are on their way while these
+// are multiplied, and the small products have a sum of their own, so that a matrix instruction waits
+// for one before it rather than for two.
 __device__ __forceinline__ floatx4 pair_product(const _Float16* p, const _Float16* q, int step_p, int step_q, int kb)
 {
-    floatx4 acc = {0, 0, 0, 0};
-    for (int k = 0; k < kb; ++k) {
-        const f16x8 ph = *reinterpret_cast<const f16x8*>(p), pl = *reinterpret_cast<const f16x8*>(p + BLOCK);
-        const f16x8 qh = *reinterpret_cast<const f16x8*>(q), ql = *reinterpret_cast<const f16x8*>(q + BLOCK);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    floatx4 acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
+    f16x8 ph = *reinterpret_cast<const f16x8*>(p), pl = *reinterpret_cast<const f16x8*>(p + BLOCK);
+    f16x8 qh = *reinterpret_cast<const f16x8*>(q), ql = *reinterpret_cast<const f16x8*>(q + BLOCK);
+    for (int k = 1; k < kb; ++k) {
         p += step_p;
         q += step_q;
+        const f16x8 nph = *reinterpret_cast<const f16x8*>(p), npl = *reinterpret_cast<const f16x8*>(p + BLOCK);
+        const f16x8 nqh = *reinterpret_cast<const f16x8*>(q), nql = *reinterpret_cast<const f16x8*>(q + BLOCK);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, low, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, low, 0, 0, 0);
+        ph = nph;
+        pl = npl;
+        qh = nqh;
+        ql = nql;
     }
-    return acc;
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, low, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, low, 0, 0, 0);
+    return acc + low;
 }
 
 __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallArgs s)
@@ -544,6 +565,16 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
     const size_t base = (size_t)blockIdx.x * s.m * s.n;
     auto index = [&](int i, int j) { return base + (s.tall ? (size_t)j * s.m + i : (size_t)i * s.n + j); };
 
+    // this wave's blocks of x and of the square
+    int x_bi[SMALL_X_BLOCKS], x_bj[SMALL_X_BLOCKS], a_bi[SMALL_A_BLOCKS], a_bj[SMALL_A_BLOCKS];
+#pragma unroll
+    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
+        x_bi[t] = (wave + t * waves) % s.mb;
+        x_bj[t] = (wave + t * waves) / s.mb;
+    }
+#pragma unroll
+    for (int t = 0; t < SMALL_A_BLOCKS; ++t) tile_of<GRAM>(wave + t * waves, 0, a_bi[t], a_bj[t]);
+
     floatx4 x[SMALL_X_BLOCKS];
     double sum = 0;
 #pragma unroll
@@ -551,7 +582,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
         const int block = wave + t * waves;
         x[t] = floatx4{0, 0, 0, 0};
         if (block < blocks) {
-            const int i = block % s.mb * 16 + (lane >> 4) * 4, j = block / s.mb * 16 + (lane & 15);
+            const int i = x_bi[t] * 16 + (lane >> 4) * 4, j = x_bj[t] * 16 + (lane & 15);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (i + r < s.m && j < s.n) {
@@ -580,8 +611,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
             if (block < blocks) {
                 f16x4 hi, lo;
                 split4(x[t], s.up_x, hi, lo);
-                if (along) store_along(xs, block % s.mb, block / s.mb, s.nb, hi, lo, lane);
-                else store_across(xs, block % s.mb, block / s.mb, s.mb, hi, lo, lane);
+                if (along) store_along(xs, x_bi[t], x_bj[t], s.nb, hi, lo, lane);
+                else store_across(xs, x_bi[t], x_bj[t], s.mb, hi, lo, lane);
             }
         }
     };
@@ -592,8 +623,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
         auto store_squares = [&](float up) {
 #pragma unroll
             for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-                int bi, bj;
-                tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+                const int bi = a_bi[t], bj = a_bj[t];
                 if (wave + t * waves < squares) {
                     f16x4 hi, lo;
                     split4(square[t], up, hi, lo);
@@ -605,8 +635,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
         const int step_a = s.mb * 2 * BLOCK;
 #pragma unroll
         for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-            int bi, bj;
-            tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+            const int bi = a_bi[t], bj = a_bj[t];
             if (wave + t * waves < squares) {
                 const floatx4 v = pair_product(xs + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.nb / 2);
 #pragma unroll
@@ -618,8 +647,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
         store_x(true);           // a is complete: nobody reads x along its columns any more
 #pragma unroll
         for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-            int bi, bj;
-            tile_of<GRAM>(wave + t * waves, 0, bi, bj);
+            const int bi = a_bi[t], bj = a_bj[t];
             if (wave + t * waves < squares) {
                 const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, as + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.mb / 2);
                 const _Float16* a = as + pair_at(bj * 16 + (lane & 15), bi * 16 + (lane >> 4) * 4, s.mb);
@@ -635,7 +663,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
         for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
             const int block = wave + t * waves;
             if (block < blocks) {
-                const int bi = block % s.mb, bj = block / s.mb;
+                const int bi = x_bi[t], bj = x_bj[t];
                 const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, s.nb * 2 * BLOCK, s.mb / 2);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[t][r] = __builtin_fmaf(s.c0, x[t][r], v[r] * down_bx);
@@ -647,7 +675,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
     for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
         const int block = wave + t * waves;
         if (block < blocks) {
-            const int i = block % s.mb * 16 + (lane >> 4) * 4, j = block / s.mb * 16 + (lane & 15);
+            const int i = x_bi[t] * 16 + (lane >> 4) * 4, j = x_bj[t] * 16 + (lane & 15);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (i + r < s.m && j < s.n) store_from_float(s.out, index(i + r, j), s.type, x[t][r]);
@@ -715,7 +743,10 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     const size_t values = (size_t)l.m * l.n;
     const size_t want = (values + 8191) / 8192;
     const int chunks = want < NORM_CHUNKS ? (int)want : NORM_CHUNKS;
-    norm_partial_kernel<<<dim3(chunks, batch), 256, 0, stream>>>(g, type, partial, values);
+    const dim3 norm_grid(chunks, batch);
+    if (type == CAKE_HIP_F32) norm_partial_kernel<CAKE_HIP_F32><<<norm_grid, 256, 0, stream>>>(static_cast<const float*>(g), partial, values);
+    else if (type == CAKE_HIP_F16) norm_partial_kernel<CAKE_HIP_F16><<<norm_grid, 256, 0, stream>>>(static_cast<const _Float16*>(g), partial, values);
+    else norm_partial_kernel<CAKE_HIP_BF16><<<norm_grid, 256, 0, stream>>>(static_cast<const __bf16*>(g), partial, values);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     normalize_kernel<<<dim3((l.nb + 3) / 4, (l.mb + 3) / 4, batch), 256, 0, stream>>>(g, type, partial, chunks, eps, up_x, x, xt[0], carried, l.m,

@@ -41,6 +41,15 @@ __device__ __forceinline__ float round_quotient(float w, float s, float inv)
     return r;
 }
 
+// a / by for a constant `by`: the product with the rounded reciprocal is within one last place, and one
+// correction by the exact remainder makes it the correctly rounded quotient (Markstein's theorem);
+// 3 operations where a division in 64 bits takes about thirty.
+__device__ __forceinline__ double quotient(double a, double by)
+{
+    const double y = 1.0 / by, q = a * y;
+    return __builtin_fma(__builtin_fma(-by, q, a), y, q);
+}
+
 __device__ __forceinline__ float larger_or_nan(float a, float b) { return (b > a || b != b) ? b : a; }
 
 __device__ __forceinline__ float as_kept(float v, int type)
@@ -55,7 +64,7 @@ __device__ __forceinline__ float as_kept(float v, int type)
 // w once (128 contiguous bytes of a row per step), writes half a byte a weight.
 template <int TYPE, int GPB>
 __global__ __launch_bounds__(256) void q4_quantize_kernel(const typename Element<TYPE>::T* __restrict__ w, unsigned char* __restrict__ q,
-                                                          Q4Layout lay, int with_zeros, bool vec)
+                                                          Q4Layout lay, int with_zeros)
 {
     typedef typename Element<TYPE>::T T;
     const int lane = threadIdx.x & 63;
@@ -68,10 +77,11 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const typename Element
     for (int i = 0; i < 4; ++i) {
         const int k = block * 128 + 32 * i + 8 * quad;
         const T* at = w + (size_t)row * lay.K + k;
-        if (row < lay.N && vec && k + 8 <= lay.K) {
-            struct alignas(16) Eight { T e[8]; } got = *reinterpret_cast<const Eight*>(at);
+        if (row < lay.N && k + 8 <= lay.K) {
+            T got[8];
+            __builtin_memcpy(got, at, sizeof got);   // 16-byte loads, which the hardware takes at any address
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = (float)got.e[e];
+            for (int e = 0; e < 8; ++e) v[i][e] = (float)got[e];
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = row < lay.N && k + e < lay.K ? (float)at[e] : 0.f;
@@ -96,7 +106,7 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const typename Element
             lo = larger_or_nan(lo, __shfl_xor(lo, step));
         }
         // range / 15 and maximum / 7, each rounded once to 32 bits, then to the type the scale is kept in
-        float s = with_zeros ? (float)(((double)hi + (double)lo) / 15.0) : (float)((double)larger_or_nan(hi, lo) / 7.0);
+        float s = with_zeros ? (float)quotient((double)hi + (double)lo, 15.0) : (float)quotient((double)larger_or_nan(hi, lo), 7.0);
         s = as_kept(s, lay.scale_type);
         // a scale so small that its reciprocal overflows: both sides of the quotient times 2^64, exactly
         const float up = s < 1e-30f ? 18446744073709551616.f : 1.f;
@@ -136,7 +146,7 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const typename Element
 // product is rounded to 32 bits and then to w's type.
 template <int TYPE, int GPB>
 __global__ __launch_bounds__(256) void q4_dequantize_kernel(const unsigned char* __restrict__ q, typename Element<TYPE>::T* __restrict__ w,
-                                                            Q4Layout lay, int with_zeros, bool vec)
+                                                            Q4Layout lay, int with_zeros)
 {
     typedef typename Element<TYPE>::T T;
     const int lane = threadIdx.x & 63;
@@ -152,22 +162,22 @@ __global__ __launch_bounds__(256) void q4_dequantize_kernel(const unsigned char*
         const size_t at = (unit * 16 + (lane & 15)) * GPB + i * GPB / 4;
         const float s = load_as_float(q + lay.scales_at, at, lay.scale_type);
         const float z = with_zeros ? load_as_float(q + lay.zeros_at, at, lay.scale_type) : 8.f;
-        struct alignas(16) Eight { T e[8]; } out;
+        T out[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float v = ((float)((codes[i] >> nibble_at(e)) & 15u) - z) * s;
             // fp16: the compiler would take product and conversion as one instruction, which rounds
             // once; the value is the product in 32 bits, whatever type it is read as
             if (TYPE == CAKE_HIP_F16) asm("" : "+v"(v));
-            out.e[e] = (T)v;
+            out[e] = (T)v;
         }
         T* to = w + (size_t)row * lay.K + k;
-        if (vec && k + 8 <= lay.K) {
-            *reinterpret_cast<Eight*>(to) = out;
+        if (k + 8 <= lay.K) {
+            __builtin_memcpy(to, out, sizeof out);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (k + e < lay.K) to[e] = out.e[e];
+                if (k + e < lay.K) to[e] = out[e];
         }
     }
 }
@@ -236,10 +246,9 @@ hipError_t launch_q4_quantize(const void* w, int w_type, void* q, const Q4Layout
 {
     const dim3 grid(q4_grid(lay)), block(256);
     unsigned char* to = static_cast<unsigned char*>(q);
-    const bool vec = lay.K % 8 == 0 && (uintptr_t)w % 16 == 0;   // every run of eight columns starts on 16 bytes
     auto go = [&](auto type, auto gpb) {
         typedef typename Element<decltype(type)::value>::T T;
-        q4_quantize_kernel<decltype(type)::value, decltype(gpb)::value><<<grid, block, 0, stream>>>(static_cast<const T*>(w), to, lay, with_zeros, vec);
+        q4_quantize_kernel<decltype(type)::value, decltype(gpb)::value><<<grid, block, 0, stream>>>(static_cast<const T*>(w), to, lay, with_zeros);
     };
     q4_for_type_and_group(w_type, lay.groups_per_block, go);
     return hipGetLastError();
@@ -249,10 +258,9 @@ hipError_t launch_q4_dequantize(const void* q, void* w, int w_type, const Q4Layo
 {
     const dim3 grid(q4_grid(lay)), block(256);
     const unsigned char* from = static_cast<const unsigned char*>(q);
-    const bool vec = lay.K % 8 == 0 && (uintptr_t)w % 16 == 0;
     auto go = [&](auto type, auto gpb) {
         typedef typename Element<decltype(type)::value>::T T;
-        q4_dequantize_kernel<decltype(type)::value, decltype(gpb)::value><<<grid, block, 0, stream>>>(from, static_cast<T*>(w), lay, with_zeros, vec);
+        q4_dequantize_kernel<decltype(type)::value, decltype(gpb)::value><<<grid, block, 0, stream>>>(from, static_cast<T*>(w), lay, with_zeros);
     };
     q4_for_type_and_group(w_type, lay.groups_per_block, go);
     return hipGetLastError();
