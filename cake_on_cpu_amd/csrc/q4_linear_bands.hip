@@ -10,19 +10,30 @@ namespace cake {
 
 namespace {
 
-// A stage of the product is 64 columns of x (32 of an fp32 x, whose three pieces take their room), a
-// band is 2 MTW tiles of 16 rows.  A band's stage is one record: the tiles as A operands, 1 KB per
-// tile, step of 32 columns and piece, and behind them for every run of columns under one scale the rows'
-// sums (times -8 where there are no zero points).
-template <int TYPE, int GROUPS_, int MTW>
+// A band is 64, 128 or 256 rows of x.  A stage of the product is a block of 128 columns, or what of it
+// fits LDS twice where three pieces of an fp32 x take their room.  A band's stage is one record: its
+// tiles of 16 rows as A operands, 1 KB per tile, step of 32 columns and piece, and behind them for every
+// run of columns under one scale the rows' sums (times -8 where there are no zero points).
+// Eight waves share the strip of 256 rows of v that a workgroup multiplies a band with.  Each takes 32
+// of them and all the band, so that no code is unpacked twice: unpacking and scaling take the vector
+// pipe 180 instructions a stage (groups of 128, 256 rows) beside 128 of the matrix pipe, and those that
+// two waves repeat, or that scale after every 64 columns, cost as much time as they take (2 x 4 waves,
+// 64 columns: 283 us for 2048 rows, 14336 x 4096; 233 this way).  256 rows of fp32, with three products a code
+// and stages of one step, go to 2 x 4 waves, which read fewer operands from LDS.
+template <int TYPE, int GROUPS_, int ROWS_>
 struct Record {
+    static constexpr int ROWS = ROWS_;
     static constexpr int PIECES = pieces_of<TYPE>();
-    static constexpr int STEPS = TYPE == CAKE_HIP_F32 ? 1 : 2;
-    static constexpr int GROUPS = GROUPS_;   // runs of columns under one scale in a stage: 2 for 16-bit x and groups of 32, else 1
-    static constexpr int TILES = 2 * MTW;
+    static constexpr int STEPS = TYPE == CAKE_HIP_F32 ? 256 / ROWS : 4;
+    static constexpr int GROUPS = GROUPS_;                                  // runs of columns under one scale in a stage: a step each for groups of 32, ...
+    static constexpr int WM = TYPE == CAKE_HIP_F32 && ROWS == 256 ? 2 : 1;  // waves along the band,
+    static constexpr int WN = 8 / WM, NT = 2 * WM;                          // along the strip, and a wave's tiles of it
+    static constexpr int TILES = ROWS / 16, MTW = TILES / WM;
     static constexpr int OPERANDS = TILES * STEPS * PIECES;                 // KB
-    static constexpr int SUMS = (TILES * 16 * GROUPS * 4 + 1023) / 1024;    // KB
-    static constexpr int KB = (OPERANDS + SUMS + 7) / 8 * 8;                 // whole rounds of eight waves
+    static constexpr int SUMS = ROWS * GROUPS;                              // floats
+    static constexpr int BYTES = OPERANDS * 1024 + SUMS * 4;
+    // stages that codes are fetched ahead: those of a narrow band are over before memory answers
+    static constexpr int CODES_AHEAD = ROWS == 256 ? 1 : 2;
 };
 
 struct BandArgs {
@@ -37,11 +48,11 @@ struct BandArgs {
 };
 
 // x into records: a wave per tile and stage.
-template <int TYPE, int GROUPS, int MTW, bool ZEROS>
+template <int TYPE, int GROUPS, int ROWS, bool ZEROS>
 __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
 {
     typedef typename Element<TYPE>::T T;
-    typedef Record<TYPE, GROUPS, MTW> R;
+    typedef Record<TYPE, GROUPS, ROWS> R;
     const int lane = threadIdx.x & 63;
     const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int tile = (int)(unit % R::TILES);
@@ -49,7 +60,7 @@ __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
     if (record >= (size_t)a.bands * a.stages) return;
     const int band = (int)(record / a.stages), stage = (int)(record - (size_t)band * a.stages);
     const int row = (band * R::TILES + tile) * 16 + (lane & 15);
-    unsigned char* to = a.records + record * (R::KB * 1024);
+    unsigned char* to = a.records + record * R::BYTES;
     float sum = 0;
 #pragma unroll
     for (int i = 0; i < R::STEPS; ++i) {
@@ -61,10 +72,10 @@ __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
             *reinterpret_cast<uintx4*>(to + ((tile * R::STEPS + i) * R::PIECES + p) * 1024 + lane * 16) = piece_of<TYPE>(v, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += (float)v[e];
-        if (i + 1 == R::STEPS || GROUPS == R::STEPS) {   // the end of a run
+        if ((i + 1) % (R::STEPS / GROUPS) == 0) {   // the end of a run
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            const int g = GROUPS == 1 ? 0 : i;
+            const int g = i / (R::STEPS / GROUPS);
             if (lane < 16)
                 reinterpret_cast<float*>(to + R::OPERANDS * 1024)[(g * R::TILES + tile) * 16 + lane] = ZEROS ? sum : -8.f * sum;
             sum = 0;
@@ -72,64 +83,76 @@ __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
     }
 }
 
-// y for bands of 32 MTW rows of x and strips of 256 rows of v: 2 x 4 waves of MTW x 4 tiles each.  A
-// band's records pass through LDS, two stages deep; codes go from memory to the registers of the wave that
-// multiplies them.  Per run of columns the matrix pipe starts from -8 times the rows' sums (or from zero,
-// and the zero point is applied behind it) and what comes out is scaled and added: for 16-bit x
-// one scaling per 2 matrix instructions (per 1 with groups of 32), which still fits beside them.
-template <int TYPE, int GROUPS, int MTW, bool ZEROS>
+// y for bands of x and strips of 256 rows of v.  A band's records pass through LDS, two stages deep, by way of
+// registers; codes go from memory to the registers of the wave that multiplies them.  Per run of
+// columns the matrix pipe starts from -8 times the rows' sums (or from zero, and the zero point is
+// applied behind it) and what comes out is scaled and added while the next run is multiplied.
+template <int TYPE, int GROUPS, int ROWS, bool ZEROS>
 __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
 {
     typedef typename Element<TYPE>::T T;
-    typedef Record<TYPE, GROUPS, MTW> R;
-    constexpr int NT = 4, LOADS = R::KB / 8, RUN = R::STEPS / GROUPS;
+    typedef Record<TYPE, GROUPS, ROWS> R;
+    constexpr int NT = R::NT, MTW = R::MTW, STEPS = R::STEPS, PIECES = R::PIECES, RUN = STEPS / GROUPS, SETS = R::CODES_AHEAD;
+    // A record is fetched in LOADS rounds of 8 KB.  Round l is put into LDS beside tile slot(l) of the stage before its
+    // own and fetched AHEAD tiles earlier: half a stage where the rounds divide by two, which
+    // needs half the registers, else a whole one.
+    constexpr int LOADS = (R::OPERANDS + 7) / 8, AHEAD = LOADS % 2 == 0 ? MTW / 2 : MTW, HELD = LOADS % 2 == 0 ? LOADS / 2 : LOADS;
+    constexpr int SUM_LOADS = (R::SUMS + 511) / 512;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quad = lane >> 4, col = lane & 15;
-    const int wm = wave >> 2, wn = wave & 3;
+    const int wm = wave / R::WN, wn = wave % R::WN;
     const int bands = a.bands, strips = (a.lay.tiles + 15) / 16;
     // bands of one strip run together, and with a multiple of eight of them each die keeps its band's x
     const int slice = (int)(blockIdx.x / (unsigned)(bands * strips)), id = (int)(blockIdx.x - (unsigned)slice * (unsigned)(bands * strips));
     const int strip = id / bands, band = id - strip * bands;
     const int s0 = (int)((long long)a.stages * slice / a.slices), s1 = (int)((long long)a.stages * (slice + 1) / a.slices);
 
-    const unsigned char* from = a.records + ((size_t)band * a.stages + s0) * (R::KB * 1024);
-    uintx4 next[LOADS];
-    auto fetch = [&](int l) {
-        next[l] = *reinterpret_cast<const uintx4*>(from + (unsigned)((l * 8 + wave) * 1024 + lane * 16));
+    const unsigned char* records = a.records + (size_t)band * a.stages * R::BYTES;
+    auto record_of = [&](int stage) { return records + (size_t)min(stage, s1 - 1) * R::BYTES; };   // past the last: fetched again, not used
+    auto slot = [](int l) { return l * MTW / LOADS; };
+    // (where the waves do not share a record out evenly, some of the last round fetch and put the same)
+    auto part = [&](int l) { return (l + 1) * 8 <= R::OPERANDS ? l * 8 + wave : min(l * 8 + wave, R::OPERANDS - 1); };
+    uintx4 next[HELD];
+    float next_sum[SUM_LOADS];
+    auto fetch = [&](int l, const unsigned char* from) {
+        next[l % HELD] = *reinterpret_cast<const uintx4*>(from + (unsigned)(part(l) * 1024 + lane * 16));
     };
     auto put = [&](int l, int to) {
-        *reinterpret_cast<uintx4*>(lds + to * (R::KB * 1024) + (l * 8 + wave) * 1024 + lane * 16) = next[l];
+        *reinterpret_cast<uintx4*>(lds + to * R::BYTES + part(l) * 1024 + lane * 16) = next[l % HELD];
     };
+    auto fetch_sums = [&](const unsigned char* from) {
+#pragma unroll
+        for (int i = 0; i < SUM_LOADS; ++i) next_sum[i] = reinterpret_cast<const float*>(from + R::OPERANDS * 1024)[min(i * 512 + (int)threadIdx.x, R::SUMS - 1)];
+    };
+    auto put_sums = [&](int to) {
+#pragma unroll
+        for (int i = 0; i < SUM_LOADS; ++i) reinterpret_cast<float*>(lds + to * R::BYTES + R::OPERANDS * 1024)[min(i * 512 + (int)threadIdx.x, R::SUMS - 1)] = next_sum[i];
+    };
+
     // Codes and scales of a stage, as they lie: scalar addresses and a lane's place behind them.  A
     // 16-bit scale is fetched as the word that holds it and taken out where it is used, so that
     // nothing waits for it here and no branch over its type breaks the loop into pieces.
     const int gpb = a.lay.groups_per_block;
     const bool wide = a.lay.scale_type == CAKE_HIP_F32, half = a.lay.scale_type == CAKE_HIP_F16;
     const int scale_bytes = wide ? 4 : 2;
-    unsigned code[NT][R::STEPS], s[NT][GROUPS], z[NT][GROUPS];
-    auto group_of = [&](int stage, int g) { return stage * R::STEPS % 4 * gpb / 4 + g; };
-    auto fetch_codes = [&](int stage) {
-        const int block = stage * R::STEPS / 4, i0 = stage * R::STEPS % 4;
+    unsigned code[SETS][NT][STEPS], s[SETS][NT][GROUPS], z[SETS][NT][GROUPS];
+    auto group_of = [&](int stage, int g) { return stage * STEPS % 4 * gpb / 4 + g; };
+    auto fetch_codes = [&](int set, int stage) {
+        stage = min(stage, s1 - 1);   // past the last: fetched again, not used
+        const int block = stage * STEPS / 4, i0 = stage * STEPS % 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int tile = min(strip * 16 + wn * NT + nt, a.lay.tiles - 1);
             const size_t unit = (size_t)tile * a.lay.blocks + block;
-            const unsigned char* at = a.q + unit * 1024 + i0 * 4;
-            if (R::STEPS == 2) {
-                const uintx2 two = *reinterpret_cast<const uintx2*>(at + (unsigned)lane * 16);
-#pragma unroll
-                for (int i = 0; i < R::STEPS; ++i) code[nt][i] = two[i & 1];
-            } else {
-                code[nt][0] = *reinterpret_cast<const unsigned*>(at + (unsigned)lane * 16);
-            }
+            __builtin_memcpy(code[set][nt], a.q + unit * 1024 + i0 * 4 + (unsigned)lane * 16, STEPS * 4);
             const unsigned char* scales = a.q + a.lay.scales_at + unit * (16 * gpb * scale_bytes);
             const unsigned char* zeros = a.q + a.lay.zeros_at + unit * (16 * gpb * scale_bytes);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const unsigned byte = (unsigned)(col * gpb + group_of(stage, g)) * scale_bytes & ~3u;
-                s[nt][g] = *reinterpret_cast<const unsigned*>(scales + byte);
-                z[nt][g] = ZEROS ? *reinterpret_cast<const unsigned*>(zeros + byte) : 0u;
+                s[set][nt][g] = *reinterpret_cast<const unsigned*>(scales + byte);
+                z[set][nt][g] = ZEROS ? *reinterpret_cast<const unsigned*>(zeros + byte) : 0u;
             }
         }
     };
@@ -146,85 +169,103 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
         for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = floatx4{0, 0, 0, 0};
     if (s0 < s1) {
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) fetch(l);
-        fetch_codes(s0);
+        for (int d = 0; d < SETS; ++d) fetch_codes(d, s0 + d);
+        fetch_sums(record_of(s0));
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) put(l, 0);
-        if (s0 + 1 < s1) from += R::KB * 1024;
+        for (int l = 0; l < LOADS; ++l) {
+            fetch(l, record_of(s0));
+            put(l, 0);
+        }
+        put_sums(0);
+        fetch_sums(record_of(s0 + 1));
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) fetch(l);
+        for (int l = 0; l < HELD; ++l) fetch(l, record_of(s0 + 1));
     }
     __syncthreads();
-    for (int stage = s0; stage < s1; ++stage) {
+    auto multiply = [&](int stage, int set) {
         const int now = (stage - s0) & 1;
-        const unsigned char* at = lds + now * (R::KB * 1024);
-        if (stage + 2 < s1) from += R::KB * 1024;
-        uintx4 b[NT][R::STEPS];
+        const unsigned char* at = lds + now * R::BYTES + lane * 16;
+        const unsigned char* at_sums = lds + now * R::BYTES + R::OPERANDS * 1024 + quad * 16;
+        const unsigned char *from1 = record_of(stage + 1), *from2 = record_of(stage + 2);
+        uintx4 b[NT][STEPS];
         float now_s[NT][GROUPS], now_z[NT][GROUPS];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int i = 0; i < R::STEPS; ++i) b[nt][i] = unpack_codes<TYPE>(code[nt][i]);
+            for (int i = 0; i < STEPS; ++i) b[nt][i] = unpack_codes<TYPE>(code[set][nt][i]);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                now_s[nt][g] = scale_in(s[nt][g], group_of(stage, g));
-                now_z[nt][g] = ZEROS ? scale_in(z[nt][g], group_of(stage, g)) : 0.f;
+                now_s[nt][g] = scale_in(s[set][nt][g], group_of(stage, g));
+                now_z[nt][g] = ZEROS ? scale_in(z[set][nt][g], group_of(stage, g)) : 0.f;
             }
         }
+        put_sums(now ^ 1);
         __builtin_amdgcn_sched_barrier(0);
-        fetch_codes(stage + 1 < s1 ? stage + 1 : stage);   // past the last stage: fetched again, not used
-        // operands one tile ahead of the products; the compiler left alone reads them all at the start
-        // and has no registers left
-        uintx4 xa[2][R::STEPS][R::PIECES];
-        floatx4 sum[2][GROUPS];
-        auto read = [&](int mt) {
-            const int tile = wm * MTW + mt;
-#pragma unroll
-            for (int i = 0; i < R::STEPS; ++i)
-#pragma unroll
-                for (int p = 0; p < R::PIECES; ++p)
-                    xa[mt & 1][i][p] = *reinterpret_cast<const uintx4*>(at + ((tile * R::STEPS + i) * R::PIECES + p) * 1024 + lane * 16);
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g)
-                sum[mt & 1][g] = *reinterpret_cast<const floatx4*>(at + R::OPERANDS * 1024 + ((g * R::TILES + tile) * 16 + quad * 4) * 4);
+        fetch_codes(set, stage + SETS);
+        fetch_sums(from2);
+        // Operands are read one tile ahead of their products, into the registers that the step before has
+        // just left; the compiler left alone reads them all at the start and has no registers for it.
+        auto operand = [&](int mt, int i, int p) {
+            return *reinterpret_cast<const uintx4*>(at + (((wm * MTW + mt) * STEPS + i) * PIECES + p) * 1024);
         };
-        read(0);
+        auto sums_of = [&](int mt, int g) { return *reinterpret_cast<const floatx4*>(at_sums + (g * R::TILES + wm * MTW + mt) * 64); };
+        uintx4 xa[STEPS][PIECES];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) xa[i][p] = operand(0, i, p);
+        floatx4 coming = sums_of(0, 0), p[2][NT], used[2];
+        auto add = [&](int mt, int g) {
+            const int turn = (mt * GROUPS + g) & 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[mt][nt][r] = __builtin_fmaf(now_s[nt][g], ZEROS ? __builtin_fmaf(-now_z[nt][g], used[turn][r], p[turn][nt][r]) : p[turn][nt][r], acc[mt][nt][r]);
+        };
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int mt = 0; mt < MTW; ++mt) {
-            if (mt + 1 < MTW) read(mt + 1);
-            // this tile's share of the next stage: out of the registers, and the stage after it in
 #pragma unroll
-            for (int l = mt * LOADS / MTW; l < (mt + 1) * LOADS / MTW; ++l) {
-                put(l, now ^ 1);
-                fetch(l);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            for (int l = 0; l < LOADS; ++l)
+                if (slot(l) == mt) put(l, now ^ 1);
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l)
+                if (slot(l) == (mt + AHEAD) % MTW) fetch(l, AHEAD < MTW && mt < AHEAD ? from1 : from2);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                floatx4 p[NT];
+                const int turn = (mt * GROUPS + g) & 1;
+                used[turn] = coming;
+                if (g + 1 < GROUPS) coming = sums_of(mt, g + 1);
+                else if (mt + 1 < MTW) coming = sums_of(mt + 1, 0);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) p[nt] = ZEROS ? floatx4{0, 0, 0, 0} : sum[mt & 1][g];
+                for (int nt = 0; nt < NT; ++nt) p[turn][nt] = ZEROS ? floatx4{0, 0, 0, 0} : used[turn];
 #pragma unroll
                 for (int i = g * RUN; i < (g + 1) * RUN; ++i)
 #pragma unroll
-                    for (int piece = R::PIECES - 1; piece >= 0; --piece)
+                    for (int piece = PIECES - 1; piece >= 0; --piece) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) p[nt] = Codes<TYPE>::mfma(xa[mt & 1][i][piece], b[nt][i], p[nt]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[mt][nt][r] = __builtin_fmaf(now_s[nt][g], ZEROS ? __builtin_fmaf(-now_z[nt][g], sum[mt & 1][g][r], p[nt][r]) : p[nt][r],
-                                                        acc[mt][nt][r]);
+                        for (int nt = 0; nt < NT; ++nt) p[turn][nt] = Codes<TYPE>::mfma(xa[i][piece], b[nt][i], p[turn][nt]);
+                        if (mt + 1 < MTW) xa[i][piece] = operand(mt + 1, i, piece);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                // the run before this one, whose products are done
+                if (g > 0) add(mt, g - 1);
+                else if (mt > 0) add(mt - 1, GROUPS - 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+        add(MTW - 1, GROUPS - 1);
         __syncthreads();
+    };
+    for (int stage = s0; stage < s1; stage += SETS) {
+        multiply(stage, 0);
+        if (SETS == 2 && stage + 1 < s1) multiply(stage + 1, SETS - 1);
     }
 
 #pragma unroll
     for (int mt = 0; mt < MTW; ++mt) {
-        const int m = ((band * 2 + wm) * MTW + mt) * 16 + quad * 4;
+        const int m = ((band * R::WM + wm) * MTW + mt) * 16 + quad * 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int n = (strip * 16 + wn * NT + nt) * 16 + col;
@@ -259,7 +300,7 @@ __global__ __launch_bounds__(256) void linear_q4_join_kernel(BandArgs a)
 
 // How a product of many rows is cut: rows per band, slices of K, and the workspace's parts.
 struct BandPlan {
-    int mtw, bands, stages, slices;
+    int rows, bands, stages, slices;
     size_t record_bytes, bytes;
 };
 
@@ -274,35 +315,35 @@ BandPlan band_plan(int M, int N, int K, int type)
         const float time = cost[i] * (float)((M + (long long)rows - 1) / rows);
         if (i == 0 || time < least) {
             least = time;
-            p.mtw = 2 << i;
+            p.rows = rows;
         }
     }
-    const int rows = 32 * p.mtw, steps = type == CAKE_HIP_F32 ? 1 : 2;
-    p.bands = (int)((M + (long long)rows - 1) / rows);
-    p.stages = (int)(((long long)K + 127) / 128) * (4 / steps);
+    const bool wide = type == CAKE_HIP_F32;
+    p.bands = (int)((M + (long long)p.rows - 1) / p.rows);
+    p.stages = (int)(((long long)K + 127) / 128) * (wide ? p.rows / 64 : 1);
     const long long groups = (((long long)N + 255) / 256) * p.bands;
-    // slices of K, of eight stages at least, until every compute unit has a workgroup
+    // slices of K, of 256 columns at least, until every compute unit has a workgroup
     p.slices = 1;
-    while (groups * (p.slices + 1) <= 256 && p.stages / (p.slices + 1) >= 8) ++p.slices;
-    // the largest record of the type: two runs a stage
-    const int kb = (2 * p.mtw * steps * (type == CAKE_HIP_F32 ? 3 : 1) + (2 * p.mtw * 16 * 2 * 4 + 1023) / 1024 + 7) / 8 * 8;
-    p.record_bytes = (size_t)p.bands * p.stages * kb * 1024;
+    while (groups * (p.slices + 1) <= 256 && p.stages / (p.slices + 1) >= (wide ? p.rows / 32 : 2)) ++p.slices;
+    // the largest record of the type: a run for each step of 32 columns
+    const size_t steps = wide ? 256 / p.rows : 4, record = (size_t)p.rows * steps * (32 * 2 * (wide ? 3 : 1) + 4);
+    p.record_bytes = ((size_t)p.bands * p.stages * record + 255) & ~(size_t)255;
     p.bytes = p.record_bytes + (p.slices > 1 ? (size_t)p.slices * M * N * sizeof(float) : 0);
     return p;
 }
 
-template <int TYPE, int GROUPS, int MTW, bool ZEROS>
+template <int TYPE, int GROUPS, int ROWS, bool ZEROS>
 hipError_t band_launch(const BandArgs& a, hipStream_t stream)
 {
-    typedef Record<TYPE, GROUPS, MTW> R;
+    typedef Record<TYPE, GROUPS, ROWS> R;
     const size_t units = (size_t)a.bands * a.stages * R::TILES;
     hipError_t e = hipSuccess;
     if (units) {   // (K == 0 is only a bias)
-        linear_q4_records_kernel<TYPE, GROUPS, MTW, ZEROS><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>(a);
+        linear_q4_records_kernel<TYPE, GROUPS, ROWS, ZEROS><<<(unsigned)((units + 3) / 4), 256, 0, stream>>>(a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    constexpr size_t LDS = (size_t)2 * R::KB * 1024;
-    auto kernel = &linear_q4_band_kernel<TYPE, GROUPS, MTW, ZEROS>;
+    constexpr size_t LDS = (size_t)2 * R::BYTES;
+    auto kernel = &linear_q4_band_kernel<TYPE, GROUPS, ROWS, ZEROS>;
     if (LDS > 64 * 1024) {
         e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
         if (e != hipSuccess) return e;
@@ -315,12 +356,23 @@ hipError_t band_launch(const BandArgs& a, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <int TYPE, int GROUPS>
-hipError_t bands_launch(const BandArgs& a, int mtw, bool zeros, hipStream_t stream)
+template <int TYPE, int ROWS>
+hipError_t rows_launch(const BandArgs& a, bool zeros, hipStream_t stream)
 {
-    if (mtw == 2) return zeros ? band_launch<TYPE, GROUPS, 2, true>(a, stream) : band_launch<TYPE, GROUPS, 2, false>(a, stream);
-    if (mtw == 4) return zeros ? band_launch<TYPE, GROUPS, 4, true>(a, stream) : band_launch<TYPE, GROUPS, 4, false>(a, stream);
-    return zeros ? band_launch<TYPE, GROUPS, 8, true>(a, stream) : band_launch<TYPE, GROUPS, 8, false>(a, stream);
+    constexpr int STEPS = Record<TYPE, 1, ROWS>::STEPS;
+    const int groups = std::max(1, STEPS * a.lay.groups_per_block / 4);
+    if (groups == 1) return zeros ? band_launch<TYPE, 1, ROWS, true>(a, stream) : band_launch<TYPE, 1, ROWS, false>(a, stream);
+    if constexpr (STEPS >= 2)
+        if (groups == 2) return zeros ? band_launch<TYPE, 2, ROWS, true>(a, stream) : band_launch<TYPE, 2, ROWS, false>(a, stream);
+    if constexpr (STEPS >= 4)
+        if (groups == 4) return zeros ? band_launch<TYPE, 4, ROWS, true>(a, stream) : band_launch<TYPE, 4, ROWS, false>(a, stream);
+    return hipErrorInvalidValue;
+}
+
+template <int TYPE>
+hipError_t bands_launch(const BandArgs& a, int rows, bool zeros, hipStream_t stream)
+{
+    return rows == 64 ? rows_launch<TYPE, 64>(a, zeros, stream) : rows == 128 ? rows_launch<TYPE, 128>(a, zeros, stream) : rows_launch<TYPE, 256>(a, zeros, stream);
 }
 
 }  // namespace
@@ -343,11 +395,8 @@ hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias
     a.bands = p.bands;
     a.stages = p.stages;
     a.slices = p.slices;
-    const bool two = type != CAKE_HIP_F32 && lay.groups_per_block == 4;
-    if (type == CAKE_HIP_F32) return bands_launch<CAKE_HIP_F32, 1>(a, p.mtw, with_zeros, stream);
-    if (type == CAKE_HIP_F16)
-        return two ? bands_launch<CAKE_HIP_F16, 2>(a, p.mtw, with_zeros, stream) : bands_launch<CAKE_HIP_F16, 1>(a, p.mtw, with_zeros, stream);
-    return two ? bands_launch<CAKE_HIP_BF16, 2>(a, p.mtw, with_zeros, stream) : bands_launch<CAKE_HIP_BF16, 1>(a, p.mtw, with_zeros, stream);
+    if (type == CAKE_HIP_F32) return bands_launch<CAKE_HIP_F32>(a, p.rows, with_zeros, stream);
+    return type == CAKE_HIP_F16 ? bands_launch<CAKE_HIP_F16>(a, p.rows, with_zeros, stream) : bands_launch<CAKE_HIP_BF16>(a, p.rows, with_zeros, stream);
 }
 
 }  // namespace cake
