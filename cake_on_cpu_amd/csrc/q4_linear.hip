@@ -127,7 +127,7 @@ struct BlockOfX<CAKE_HIP_F32, REGS> {
 // first result register and REGS registers cover 4 REGS rows: with one token the scale costs two
 // operations per group instead of eight.
 template <int TYPE, int GPB, bool WIDE, int REGS, int NT>
-__global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
+__global__ __launch_bounds__(1024 / NT) void linear_q4_stream_kernel(StreamArgs a)
 {
     typedef typename Element<TYPE>::T T;
     constexpr int PIECES = pieces_of<TYPE>();
@@ -150,8 +150,9 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
     struct Held {
         uintx4 code[NT];
         GroupValues<GPB, WIDE> s[NT], z[NT];
-        BlockOfX<TYPE, REGS> x;
     } held[DEPTH];
+    constexpr int X_SETS = GPB == 4 ? 2 : DEPTH;   // four groups' scales leave registers for the next turn's x only
+    BlockOfX<TYPE, REGS> x[X_SETS];
     // addresses are scalars that move on by the waves' number of blocks, and a lane's place in a block
     constexpr int SCALE_BYTES = 16 * GPB * (WIDE ? 4 : 2);
     const bool half = a.lay.scale_type == CAKE_HIP_F16;
@@ -175,9 +176,11 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
                 scale_at[nt] += waves * SCALE_BYTES;
                 zero_at[nt] += waves * SCALE_BYTES;
             }
-            h.x.fetch(static_cast<const T*>(a.x), a.M, K, fetched, lane, my_row);
         }
         fetched += waves;
+    };
+    auto fetch_x = [&](int set, int block) {
+        if (block < blocks) x[set].fetch(static_cast<const T*>(a.x), a.M, K, block, lane, my_row);
     };
 
     floatx4 acc[NT];
@@ -187,8 +190,8 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) ones[i] = Codes<TYPE>::ONES;
 
-    auto multiply = [&](const Held& h) {
-        h.x.to_lds(mine, lane);
+    auto multiply = [&](const Held& h, const BlockOfX<TYPE, REGS>& bx) {
+        bx.to_lds(mine, lane);
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
             floatx4 p[NT], sum = floatx4{0, 0, 0, 0};
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
             for (int nt = 0; nt < NT; ++nt) p[nt] = floatx4{0, 0, 0, 0};
 #pragma unroll
             for (int i = g * SG; i < (g + 1) * SG; ++i) {
-                const uintx4 xa = h.x.operand(i, mine_row, real);
+                const uintx4 xa = bx.operand(i, mine_row, real);
                 sum = Codes<TYPE>::mfma(xa, ones, sum);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) p[nt] = Codes<TYPE>::mfma(xa, unpack_codes<TYPE>(h.code[nt][i]), p[nt]);
@@ -207,16 +210,20 @@ __global__ __launch_bounds__(1024) void linear_q4_stream_kernel(StreamArgs a)
 #pragma unroll
                 for (int r = 0; r < REGS; ++r) acc[nt][r] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[r], p[nt][r]), acc[nt][r]);
             }
+            if (GPB == 4) __builtin_amdgcn_sched_barrier(0);   // all groups' codes unpacked at once have no room in registers
         }
     };
 
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) fetch(held[d]);
+#pragma unroll
+    for (int d = 0; d < X_SETS - 1; ++d) fetch_x(d, wave + d * waves);
     for (int block = wave; block < blocks;) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             if (block < blocks) {
-                multiply(held[d]);
+                fetch_x((d + X_SETS - 1) % X_SETS, block + (X_SETS - 1) * waves);
+                multiply(held[d], x[d % X_SETS]);
                 fetch(held[d]);
             }
             block += waves;
