@@ -172,9 +172,11 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
         for (int d = 0; d < SETS; ++d) fetch_codes(d, s0 + d);
         fetch_sums(record_of(s0));
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            fetch(l, record_of(s0));
-            put(l, 0);
+        for (int l0 = 0; l0 < LOADS; l0 += HELD) {
+#pragma unroll
+            for (int l = l0; l < l0 + HELD; ++l) fetch(l, record_of(s0));
+#pragma unroll
+            for (int l = l0; l < l0 + HELD; ++l) put(l, 0);
         }
         put_sums(0);
         fetch_sums(record_of(s0 + 1));
@@ -304,32 +306,46 @@ struct BandPlan {
     size_t record_bytes, bytes;
 };
 
-BandPlan band_plan(int M, int N, int K, int type)
+// Microseconds of 128 columns of a band on a busy device, for runs of 128 columns without zero points and for runs of
+// 32 with them (one scaling operation an element and 128 columns against eight); measured on 4096 x 14336 and 14336 x 4096.
+// Wide bands need fewer passes over the codes; of fp32 and of many scalings they have no registers to spare.
+struct BandCost {
+    int rows;
+    float least[2], most[2];   // of 16-bit and fp32 x
+};
+constexpr BandCost BAND_COSTS[] = {{64, {1.3f, 2.6f}, {3.0f, 4.8f}}, {128, {2.0f, 5.3f}, {4.2f, 6.6f}}, {256, {4.0f, 11.8f}, {10.7f, 12.4f}}};
+enum { BAND_CUS = 256, BAND_MAX_SLICES = 24 };   // fixed, so that sizes alone decide on the workspace and the order of the sums
+
+BandPlan band_plan(int M, int N, int K, int type, int groups_per_block, bool zeros)
 {
-    BandPlan p;
-    // time of a band next to one of 256 rows: a narrow one leaves the matrix pipe idle behind its codes
-    const float cost[3] = {0.40f, 0.60f, 1.f};
-    float least = 0;
-    for (int i = 0; i < 3; ++i) {
-        const int rows = 64 << i;
-        const float time = cost[i] * (float)((M + (long long)rows - 1) / rows);
-        if (i == 0 || time < least) {
-            least = time;
-            p.rows = rows;
+    BandPlan best{};
+    const int wide = type == CAKE_HIP_F32;
+    const float scalings = (float)(groups_per_block * (zeros ? 2 : 1));
+    const int blocks = (int)(((long long)K + 127) / 128);
+    float least_us = 0;
+    for (const BandCost& c : BAND_COSTS) {
+        const float block_us = c.least[wide] + (scalings - 1) / 7 * (c.most[wide] - c.least[wide]);
+        const int bands = (int)((M + (long long)c.rows - 1) / c.rows);
+        const long long groups = (((long long)N + 255) / 256) * bands;
+        for (int s = 1; s <= BAND_MAX_SLICES && (s == 1 || (groups * s <= 2 * BAND_CUS && s <= blocks)); ++s) {
+            const float rounds = (float)((groups * s + BAND_CUS - 1) / BAND_CUS);
+            // a workgroup's beginning and end, and for slices another launch and a pass over their sums
+            float us = rounds * (block_us * (float)((blocks + s - 1) / s) + 3.f);
+            if (s > 1) us += 3.f + (float)s * (float)M * (float)N * 8 / 6e6f;
+            if (best.rows == 0 || us < least_us) {
+                least_us = us;
+                best.rows = c.rows;
+                best.bands = bands;
+                best.slices = s;
+            }
         }
     }
-    const bool wide = type == CAKE_HIP_F32;
-    p.bands = (int)((M + (long long)p.rows - 1) / p.rows);
-    p.stages = (int)(((long long)K + 127) / 128) * (wide ? p.rows / 64 : 1);
-    const long long groups = (((long long)N + 255) / 256) * p.bands;
-    // slices of K, of 256 columns at least, until every compute unit has a workgroup
-    p.slices = 1;
-    while (groups * (p.slices + 1) <= 256 && p.stages / (p.slices + 1) >= (wide ? p.rows / 32 : 2)) ++p.slices;
+    best.stages = blocks * (wide ? best.rows / 64 : 1);
     // the largest record of the type: a run for each step of 32 columns
-    const size_t steps = wide ? 256 / p.rows : 4, record = (size_t)p.rows * steps * (32 * 2 * (wide ? 3 : 1) + 4);
-    p.record_bytes = ((size_t)p.bands * p.stages * record + 255) & ~(size_t)255;
-    p.bytes = p.record_bytes + (p.slices > 1 ? (size_t)p.slices * M * N * sizeof(float) : 0);
-    return p;
+    const size_t steps = wide ? 256 / best.rows : 4, record = (size_t)best.rows * steps * (32 * 2 * (wide ? 3 : 1) + 4);
+    best.record_bytes = ((size_t)best.bands * best.stages * record + 255) & ~(size_t)255;
+    best.bytes = best.record_bytes + (best.slices > 1 ? (size_t)best.slices * M * N * sizeof(float) : 0);
+    return best;
 }
 
 template <int TYPE, int GROUPS, int ROWS, bool ZEROS>
@@ -377,12 +393,18 @@ hipError_t bands_launch(const BandArgs& a, int rows, bool zeros, hipStream_t str
 
 }  // namespace
 
-size_t linear_q4_bands_workspace(int M, int N, int K, int type) { return band_plan(M, N, K, type).bytes; }
+size_t linear_q4_bands_workspace(int M, int N, int K, int type)
+{
+    size_t most = 0;   // whatever the weights' groups and zero points
+    for (int per_block : {1, 2, 4})
+        for (bool zeros : {false, true}) most = std::max(most, band_plan(M, N, K, type, per_block, zeros).bytes);
+    return most;
+}
 
 hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
                                   bool with_zeros, void* workspace, hipStream_t stream)
 {
-    const BandPlan p = band_plan(M, lay.N, lay.K, type);
+    const BandPlan p = band_plan(M, lay.N, lay.K, type, lay.groups_per_block, with_zeros);
     BandArgs a{};
     a.x = x;
     a.q = static_cast<const unsigned char*>(q);
