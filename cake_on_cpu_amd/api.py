@@ -628,7 +628,8 @@ def linear_q4_workspace(M, N, K, dtype="float32") -> int:
 
 def linear_q4_forward(x, q: Q4Weight, bias, y, M, workspace=None, timed=True) -> float:
     """y[M][N] = x[M][K] . v[N][K]^T + bias[N] (bias may be None); x, bias and y of one element type.
-    workspace: a uint8 device tensor of linear_q4_workspace bytes, or None for the library's own.
+    workspace: a uint8 device tensor of linear_q4_workspace bytes, or None for the library's own
+    (calls on several streams at once need one each).
     Returns seconds (0 with timed=False, which makes the call asynchronous on device operands)."""
     t = element_type(x.dtype)
     N, K = q.N, q.K
@@ -658,7 +659,8 @@ def orthogonalize_workspace(batch, rows, cols) -> int:
 def orthogonalize(g, out, batch, rows, cols, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, workspace=None, timed=True) -> float:
     """Newton-Schulz iterations on g[batch][rows][cols] into out (of g's element type; may be g):
     x = g / (|g| + eps), then `steps` times a = x x^T, x = c0 x + (c1 a + c2 a a) x.
-    Returns seconds (0 with timed=False)."""
+    workspace: a uint8 device tensor of orthogonalize_workspace bytes, or None for the library's own
+    (calls on several streams at once need one each).  Returns seconds (0 with timed=False)."""
     t = element_type(g.dtype)
     _need(g, batch * rows * cols, "g")
     _need(out, batch * rows * cols, "out")

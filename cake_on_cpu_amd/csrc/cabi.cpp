@@ -2276,7 +2276,7 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
 
 size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type)
 {
-    if (linear_dims_ok(M, N, K) || !element_type_ok(type)) return 0;
+    if (linear_dims_ok(M, N, K) || !element_type_ok(type) || M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00) return 0;
     return linear_q4_workspace(M, N, K, type);
 }
 
@@ -2288,6 +2288,7 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
     if (st) return st;
     if ((st = q4_args_ok(N, K, group, scale_type))) return st;
     if (!element_type_ok(type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", type);
+    if (M > 0x7FFFFF00) return fail(CAKE_HIP_ERR_RANGE, "%d rows of x", M);   // padded to whole bands in 32-bit arithmetic
     if (M == 0 || N == 0) return CAKE_HIP_OK;
     if (!y || (K > 0 && (!x || !q))) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
     if ((st = ensure_init())) return st;
@@ -2360,7 +2361,9 @@ static int orthogonalize_scales(int steps, double c0, double c1, double c2, Orth
 static int orthogonalize_dims_ok(int batch, int rows, int cols)
 {
     if (batch < 0 || rows < 0 || cols < 0) return fail(CAKE_HIP_ERR_ARG, "negative dimension");
-    if (!fits_int((double)rows * cols)) return fail(CAKE_HIP_ERR_RANGE, "matrix of %dx%d exceeds 2^31 elements", rows, cols);
+    // sides are padded to whole blocks in 32-bit arithmetic
+    if (!fits_int((double)rows * cols) || rows > 0x7FFFFF00 || cols > 0x7FFFFF00)
+        return fail(CAKE_HIP_ERR_RANGE, "matrix of %dx%d exceeds 2^31 elements", rows, cols);
     if (batch > 65535) return fail(CAKE_HIP_ERR_RANGE, "batch of %d matrices (65535 at most)", batch);
     return CAKE_HIP_OK;
 }

@@ -164,6 +164,7 @@ class cake_linear_q4_function(torch.autograd.Function):
         return _forward_q4(data.detach().contiguous(), q, None if bias is None else bias.detach().contiguous())
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         q, M = ctx.q, grad_output.size(0)
         g = grad_output.detach().float().contiguous()
@@ -264,7 +265,7 @@ class cake_muon(torch.optim.Optimizer):
         for group in self.param_groups:
             alike = {}
             for w in group["params"]:
-                if w.grad is None:
+                if w.grad is None or w.numel() == 0:
                     continue
                 state = self.state[w]
                 if "momentum" not in state:

@@ -147,7 +147,7 @@ def test_in_place_views_and_host_operands():
 
 def test_captured_updates_side_by_side():
     gen = torch.Generator(device="cuda").manual_seed(1)
-    for shape in ((3, 60, 100), (300, 200)):
+    for shape in ((3, 60, 100), (300, 200), (2100, 2300)):
         gs = [torch.randn(*shape, device="cuda", generator=gen) for _ in range(2)]
         streams = [torch.cuda.Stream() for _ in range(2)]
         for g, st in zip(gs, streams):
@@ -234,3 +234,32 @@ def test_a_layer_is_trained_held_in_4_bits_and_served():
         want = x.double().cpu() @ v.t() + layer.bias.double().cpu()
         mass = x.double().cpu().abs() @ (step[:, torch.arange(192) // 64] * 31).t() + layer.bias.double().cpu().abs()
         assert bool(((held(x).double().cpu() - want).abs() <= (16 * 2 + 48) * 2.0 ** -24 * mass).all()), rows
+
+
+def test_a_batch_beyond_4_gb():
+    """2.2 billion values in one call: the last matrix as good as the first."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB of device memory")
+    batch, m, n = 530, 2048, 2048
+    g = torch.empty(batch, m, n, dtype=torch.bfloat16, device="cuda").normal_(0, 1e-3, generator=torch.Generator(device="cuda").manual_seed(1))
+    print("orthogonalize batch beyond 4 GB", flush=True)
+    out = tl.orthogonalize(g, steps=2)
+    for i in (0, batch - 1):
+        x = g[i].double()
+        x = x / (x.norm() + 1e-7)
+        bar = float(x.norm()) * 3.4445 ** 2
+        for step in (1, 2):
+            a = x @ x.t().contiguous()
+            x = USUAL[0] * x + (USUAL[1] * a + USUAL[2] * (a @ a)) @ x
+            bar += float(x.norm()) * 3.4445 ** (2 - step)
+        far = ((out[i].double() - x).abs() - 2.0 ** -8 * x.abs()).clamp(min=0)
+        assert float(far.norm()) <= 32 * 2.0 ** -24 * bar * (1 + 2.0 ** -7), i
+    torch.cuda.empty_cache()
+
+
+def test_optimiser_leaves_empty_and_untouched_parameters_alone():
+    a, b, c = (torch.nn.Parameter(torch.ones(s, device="cuda")) for s in ((4, 6), (0, 6), (5, 3)))
+    opt = tl.cake_muon([a, b, c])
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    assert bool((c == 1).all()) and not bool((a == 1).any())

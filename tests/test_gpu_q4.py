@@ -297,3 +297,37 @@ def test_refusals_on_the_device():
     torch.cuda.synchronize()
     assert bool((y == 7).all())
     del host
+
+
+def test_operands_beyond_4_gb():
+    """Weights of 4.2 GB (2.1 billion, as many as an operand may have): the last rows as good as the first."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    N, K = 65536, 32000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(N, K, dtype=torch.bfloat16, device="cuda").normal_(0, 0.02, generator=gen)
+    q = tl.quantize_q4(w, 64, True, torch.bfloat16)
+    rows = torch.cat([torch.arange(0, 40), torch.arange(N - 40, N)]).cuda()
+    v = _quantized64(w[rows].cpu(), 64, True, torch.bfloat16)
+    back = tl.dequantize_q4(q, torch.bfloat16)
+    assert torch.equal(back[rows].cpu(), v.float().bfloat16())
+    del back
+    for M in (1, 40):
+        x = torch.randn(M, K, device="cuda", generator=gen)
+        print(f"linear_q4 beyond 4 GB M={M}", flush=True)
+        y = tl.forward_q4(x, q)[:, rows]
+        # codes and zero points are at most 15, so s (code + zero) is at most 30 s, and s at most a fifteenth of twice the largest weight
+        mass = x.double().cpu().abs().sum(1, keepdim=True) * (30 * 2 / 15 * float(w.abs().max()) * (1 + 2.0 ** -7))
+        assert bool(((y.double().cpu() - x.double().cpu() @ v.t()).abs() <= (16 * (K // 128) + 48) * 2.0 ** -24 * mass).all())
+
+
+def test_an_input_of_tiny_values():
+    """Products of values down to 2^-100 keep their relative accuracy; below that pieces leave bf16's normal range."""
+    N, K, M = 40, 256, 3
+    packed, s, z, v64, mass = _weights(N, K, 64, True, torch.float32, 4)
+    q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda(), K, 64)
+    for rows in (M, 30):
+        x = torch.randn(rows, K, generator=torch.Generator().manual_seed(4)) * 2.0 ** -100
+        want = x.double() @ v64.t()
+        tol = (16 * 2 + 48) * 2.0 ** -24 * (x.double().abs() @ mass.t())
+        assert bool(((tl.forward_q4(x.cuda(), q).double().cpu() - want).abs() <= tol).all()), rows

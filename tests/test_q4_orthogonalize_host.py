@@ -53,6 +53,7 @@ def test_q4_null_type_and_range():
         assert lib.cake_hip_q4_size(N, K, 32, F32, 0) == 0
         assert lib.cake_hip_q4_quantize(b, F32, b, N, K, 32, F32, 0, None, None) == _lib.ERR_RANGE
     assert lib.cake_hip_linear_q4_forward(b, b, None, b, F32, 1 << 20, 8, 4096, 32, F32, 0, None, None, None) == _lib.ERR_RANGE
+    assert lib.cake_hip_linear_q4_forward(b, b, None, b, F32, 0x7FFFFF80, 1, 1, 32, F32, 0, None, None, None) == _lib.ERR_RANGE
     # nothing to do: no device is asked for
     assert lib.cake_hip_linear_q4_forward(None, None, None, None, F32, 0, 8, 8, 32, F32, 0, None, None, None) == _lib.OK
     assert lib.cake_hip_q4_quantize(None, F32, None, 0, 8, 32, F32, 0, None, None) == _lib.OK
@@ -69,6 +70,7 @@ def test_orthogonalize_refuses():
         assert _orth(**bad) == _lib.ERR_ARG, bad
     assert _orth(batch=65536) == _lib.ERR_RANGE
     assert _orth(rows=65536, cols=32768) == _lib.ERR_RANGE
+    assert _orth(rows=1, cols=0x7FFFFFF0) == _lib.ERR_RANGE and _orth(rows=0x7FFFFFF0, cols=1) == _lib.ERR_RANGE
     assert _orth(batch=0) == _lib.OK and _orth(rows=0) == _lib.OK and _orth(cols=0, g=False) == _lib.OK
     # polynomials that drive singular values away from 1 without bound
     assert _orth(c=(40.0, 0.0, 0.0)) == _lib.ERR_ARG
