@@ -4,15 +4,15 @@
 //
 // All products run on the 16-bit matrix pipe at 32-bit accuracy.  A value v is kept as two fp16
 // numbers, hi = fp16(v 2^e) and lo = fp16(v 2^e - hi): 11 significant bits each and the sign of lo
-// make 2^-24 of relative error, and the power of two e keeps both parts in fp16's range (the
+// leave at most 2^-23 of the value, and the power of two e keeps both parts in fp16's range (the
 // iteration's values are bounded by its coefficients, so e is known beforehand).  A product is then
 // hi hi + hi lo + lo hi -- three matrix instructions where the fp32 ones, at a sixteenth of the rate,
-// would take the time of sixteen -- summed in 32 bits; lo lo is below 2^-24 of the product.  The
-// floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39 of the largest a value can be.
+// would take the time of sixteen -- summed in 32 bits; lo lo is at most 2^-22 of the product, of
+// either sign.  The floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39.
 // b is kept without c0 I, and while four or more steps follow x is carried in fp32 beside its
 // pairs: early steps are little more than x = c0 x, and what is lost of a small singular value there
-// is enlarged by every later step (final error on a 1024 x 1024 gradient: 4.2e-7 carried to the end, 5.2e-7 so, 7.8e-7 never;
-// fp32 products give 1.3e-6).
+// is enlarged by every later step (final error on a 1024 x 1024 gradient: 4.2e-7 carried to the end,
+// 5.2e-7 so, 7.8e-7 never; fp32 products give 1.3e-6).
 //
 // a and a a are symmetric: only tiles on and above the diagonal are computed and written twice.
 //
@@ -514,7 +514,7 @@ size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
 // compute unit together (sides up to 128 x 160, 64 x 560, 32 x 1200).  x stays in registers in fp32, in
 // blocks as they come out of the matrix pipe; its pairs are written to LDS along its columns for
 // a = x x^T and then, over them, along its rows for b x.  Launches of a product each cost 5 to 6 us
-// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 49 us in one.
+// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 45 us in one.
 enum { SMALL_WAVES = 16, SMALL_X_BLOCKS = 10, SMALL_A_BLOCKS = 3 };   // blocks a wave holds of x and of the square
 
 struct SmallArgs {

@@ -443,11 +443,12 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
                            void* stream, double* seconds);
 
 /* y[M][N] = x[M][K] . v[N][K]^T (+ bias[N] on every row when bias != NULL); x, bias and y are of `type`.
- * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and zero points are applied to a
- * run's sum in fp32, and y is rounded once.  The order of the sums depends on the sizes alone.  An infinity in x
- * may come out as NaN in that row of y.  workspace: device memory of cake_hip_linear_q4_workspace bytes
- * (0 for a few rows of x), 16-byte aligned, or NULL for a buffer of the context's own; calls that
- * overlap (two streams, two captured graphs) need workspaces of their own. */
+ * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and
+ * zero points are applied to a run's sums in fp32, and y is rounded once.  The order of the sums depends
+ * on the sizes, types and groups alone.  An infinity in x may come out as NaN in that row of y.  K == 0
+ * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 16 rows of
+ * x, 5 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
+ * streams, two captured graphs) need workspaces of their own. */
 size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type);
 int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, void* y, int type, int M, int N, int K,
                                int group, int scale_type, int with_zeros, void* workspace, void* stream,
@@ -463,11 +464,11 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
  * steps >= 1.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
  * count as they are, the result is rounded once).  Singular values start in 0..1; coefficients whose
  * polynomial takes them beyond 1000 within `steps` are refused (CAKE_HIP_ERR_ARG).  x is kept to
- * 2^-24 of each value and no finer than 2^-39 (for the coefficients above), so a g whose
+ * 2^-23 of each value and no finer than 2^-39 (for the coefficients above), so a g whose
  * norm lies below about 1e-4 eps loses relative accuracy.  A matrix of zeros gives zeros; one that holds a NaN
  * or an infinity gives NaN and leaves the rest of the batch alone.
- * workspace: device memory of cake_hip_orthogonalize_workspace bytes, 256-byte aligned, or NULL for a
- * buffer of the context's own; calls that overlap need workspaces of their own. */
+ * workspace: device memory of cake_hip_orthogonalize_workspace bytes (0 for small matrices), 256-byte
+ * aligned, or NULL for a buffer of the context's own; calls that overlap need workspaces of their own. */
 size_t cake_hip_orthogonalize_workspace(int batch, int rows, int cols);
 int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0,
                            double c1, double c2, double eps, void* workspace, void* stream, double* seconds);

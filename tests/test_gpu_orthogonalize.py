@@ -1,8 +1,8 @@
 """GPU checks of orthogonalize (Newton-Schulz iterations) and of the optimiser on it, against the definition
 in 64 bits.
 
-The bar.  One iteration commits an error of at most C 2^-24 of its result's Frobenius norm -- each kept value and
-each product to 2^-24, sums over a side of which the random part grows with its root; C = 32 allows for sides up to
+The bar.  One iteration commits an error of at most C 2^-24 of its result's Frobenius norm -- each kept value to
+2^-23 and each product to 2^-22, of either sign, sums over a side of which the random part grows with its root; C = 32 allows for sides up to
 some hundreds -- and every later iteration enlarges a perturbation by at most the largest of |p(s)| / s
 and |p'(s)| over the singular values it meets, L = 3.4445 for the usual coefficients (both at 0) and 1.5 for
 (1.5, -0.5, 0).  So |x - x64|_F <= C 2^-24 sum_i |x_i|_F L^(steps - i), plus half a step of the type per entry.
