@@ -2305,10 +2305,11 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
     if (bias && (st = any_in(bias, (size_t)N * b, 2, true, &bo, "bias"))) return st;
     if ((st = any_in(y, (size_t)M * N * b, 3, false, &yo, "y"))) return st;
     void* ws = nullptr;
-    if ((st = workspace_of(workspace, linear_q4_workspace(M, N, K, type), 16, cur().linear_q4, &ws))) return st;
+    const size_t need = linear_q4_workspace(M, N, K, type);   // none: the rows are few and the codes are streamed
+    if ((st = workspace_of(workspace, need, 16, cur().linear_q4, &ws))) return st;
     Timer timer(stream, seconds);
     if ((st = timer.start())) return st;
-    st = timer.family(M <= 64 ? 2 : 0, [&] {
+    st = timer.family(need ? 0 : 2, [&] {
         return launch_linear_q4(xo.dev, qo.dev, bias ? bo.dev : nullptr, yo.dev, type, M, lay, with_zeros != 0, ws, stream);
     });
     if (st) return st;

@@ -182,8 +182,19 @@ __global__ __launch_bounds__(256) void q4_dequantize_kernel(const unsigned char*
     }
 }
 
+// Eight columns of a checkpoint's row (byte j: column 2 j low, 2 j + 1 high) as a dword of the packed form
+__device__ __forceinline__ unsigned reorder_nibbles(unsigned w)
+{
+    const unsigned even = w & 0x0F0F0F0Fu, odd = w >> 4 & 0x0F0F0F0Fu;   // columns 0 2 4 6 and 1 3 5 7, a byte each
+    const unsigned low = (even & 0x00FFu) | (odd & 0x00FFu) << 8 | (even & 0xFF00u) << 8 | (odd & 0xFF00u) << 16;   // 0 1 2 3
+    const unsigned high = (even >> 16 & 0x00FFu) | (odd >> 16 & 0x00FFu) << 8 | (even >> 16 & 0xFF00u) << 8 | (odd >> 16 & 0xFF00u) << 16;
+    return low | high << 4;
+}
+
 // codes[N][(K + 1) / 2] (byte j of a row: column 2 j in the low nibble, 2 j + 1 in the high one), scales and
-// zero points [N][groups] into the packed form.  Runs once per weight: plain byte loads.
+// zero points [N][groups] into the packed form.  A lane fetches 32 columns of its row, 16 bytes at any
+// address, so that the four lanes of a row read 64 bytes in a row; what it keeps is its eight of
+// each of the four steps, a 4 x 4 transposition among them.
 template <int GPB>
 __global__ __launch_bounds__(256) void q4_pack_kernel(const unsigned char* __restrict__ codes, const void* __restrict__ scales,
                                                       const void* __restrict__ zeros, unsigned char* __restrict__ q, Q4Layout lay)
@@ -193,19 +204,35 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const unsigned char* __res
     if (unit >= (size_t)lay.tiles * lay.blocks) return;
     const int tile = (int)(unit / lay.blocks), block = (int)(unit - (size_t)tile * lay.blocks);
     const int row = tile * 16 + (lane & 15), quad = lane >> 4;
-    const unsigned char* from = codes + (size_t)row * ((lay.K + 1) / 2);
+    const int k0 = block * 128 + 32 * quad;
+    unsigned w[4] = {0, 0, 0, 0};
+    if (row < lay.N) {
+        const unsigned char* from = codes + (size_t)row * ((lay.K + 1) / 2) + k0 / 2;
+        if (k0 + 32 <= lay.K) {
+            __builtin_memcpy(w, from, 16);
+        } else {
+            for (int k = k0; k < lay.K; ++k) {   // (a last column in a byte of its own leaves the byte's other half out)
+                const unsigned code = (from[(k - k0) >> 1] >> (4 * (k & 1))) & 15u;
+                const int at = k - k0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] |= at >> 3 == j ? code << (4 * (at & 7)) : 0u;
+            }
+        }
+    }
+    // w[j] of quarter i is columns 32 i + 8 j; wanted in quarter j's w[i]
+    auto swap = [&](unsigned& a, unsigned& b, int across) {
+        const bool upper = (lane & across) != 0;
+        const unsigned got = __shfl_xor(upper ? a : b, across);
+        a = upper ? got : a;
+        b = upper ? b : got;
+    };
+    swap(w[0], w[1], 16);
+    swap(w[2], w[3], 16);
+    swap(w[0], w[2], 32);
+    swap(w[1], w[3], 32);
     uintx4 out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        unsigned word = 0;
-        const int k0 = block * 128 + 32 * i + 8 * quad;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int k = k0 + e;
-            if (row < lay.N && k < lay.K) word |= (unsigned)((from[k >> 1] >> (4 * (k & 1))) & 15) << nibble_at(e);
-        }
-        out[i] = word;
-    }
+    for (int i = 0; i < 4; ++i) out[i] = reorder_nibbles(w[i]);
     *reinterpret_cast<uintx4*>(q + unit * 1024 + lane * 16) = out;
     if (quad == 0) {
         const int groups = (lay.K + 128 / GPB - 1) / (128 / GPB);
