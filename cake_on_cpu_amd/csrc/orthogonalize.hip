@@ -306,13 +306,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void pair_gemm_kernel(PairGemm g)
     const char* from_p = reinterpret_cast<const char*>(p);     // the same for every lane: addresses are scalars
     const char* from_q = reinterpret_cast<const char*>(q);
     const size_t step_p = (size_t)g.ib * 4 * BLOCK, step_q = (size_t)g.jb * 4 * BLOCK;
-    from_p += k0 * step_p;
-    from_q += k0 * step_q;
-    unsigned at_part[LOADS];
+    from_p += k0 * step_p + (size_t)ti * BI * 4 * BLOCK;
+    from_q += k0 * step_q + (size_t)tj * BJ * 4 * BLOCK;
+    unsigned at_part[LOADS];   // within the tile: 32 bits, however long the side
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
         const int part = l * WAVES + wave, t = part >> 1;
-        const int block = l < P_LOADS ? min(ti * BI + t, g.ib - 1) : min(tj * BJ + t - BI, g.jb - 1);
+        const int block = l < P_LOADS ? min(t, g.ib - 1 - ti * BI) : min(t - BI, g.jb - 1 - tj * BJ);
         at_part[l] = (unsigned)block * 4 * BLOCK + (part & 1) * 2 * BLOCK + lane * 16;
     }
     f16x8 next[LOADS];

@@ -263,3 +263,22 @@ def test_optimiser_leaves_empty_and_untouched_parameters_alone():
     a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
     opt.step()
     assert bool((c == 1).all()) and not bool((a == 1).any())
+
+
+def test_a_row_of_more_than_2_to_the_25_columns():
+    """Operands whose block rows pass 32 bits.  One row of norm 1 stays a multiple of itself, x (c0 + b) in every step; its
+    pair, b's and the sum are off by 2^-23 each, relative to |c0| + |b|, which is at most 10 |c0 + b| on the way of 1."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    n = (1 << 25) + (1 << 20) + 5
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for shape in ((1, n), (n, 1)):
+        g = torch.randn(shape, device="cuda", generator=gen)
+        print(f"orthogonalize {shape}", flush=True)
+        out = tl.orthogonalize(g).double().flatten()
+        unit = g.double().flatten() / g.double().norm()
+        along = float(out @ unit)
+        assert 0.6 < along < 1.3
+        assert float((out - along * unit).abs().max()) <= 5 * 10 * 3 * 2.0 ** -23 * 1.3 * float(unit.abs().max())
+        del g, out, unit
+    torch.cuda.empty_cache()
