@@ -2177,14 +2177,17 @@ static int workspace_of(void* given, size_t bytes, size_t align, DeviceBuffer& b
 
 static bool element_type_ok(int type) { return type == CAKE_HIP_F32 || type == CAKE_HIP_F16 || type == CAKE_HIP_BF16; }
 
+// The sides of which a launch takes 4 threads each, and those (rows of x) of which it takes 8.
+enum { MOST_ROWS = 0x3FFFFF00, MOST_INPUTS = 0x1FFFFF00 };
+
 static int q4_args_ok(int N, int K, int group, int scale_type)
 {
     if (N < 0 || K < 0) return fail(CAKE_HIP_ERR_ARG, "negative dimension");
     if (group != 32 && group != 64 && group != 128) return fail(CAKE_HIP_ERR_ARG, "group of %d weights (32, 64 or 128)", group);
     if (!element_type_ok(scale_type)) return fail(CAKE_HIP_ERR_ARG, "unknown scale type %d", scale_type);
-    // rows and columns are padded to whole tiles in 32-bit arithmetic
-    if (!fits_int((double)N * K) || N > 0x7FFFFF00 || K > 0x7FFFFF00)
-        return fail(CAKE_HIP_ERR_RANGE, "weights of %dx%d exceed 2^31 elements", N, K);
+    // columns are padded to whole blocks in 32-bit arithmetic, and a launch has less than 2^32 threads
+    if (!fits_int((double)N * K) || N > MOST_ROWS || K > 0x7FFFFF00)
+        return fail(CAKE_HIP_ERR_RANGE, "weights of %dx%d exceed 2^31 elements or 2^30 rows", N, K);
     return CAKE_HIP_OK;
 }
 
@@ -2276,7 +2279,7 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
 
 size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type)
 {
-    if (linear_dims_ok(M, N, K) || !element_type_ok(type) || M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00) return 0;
+    if (linear_dims_ok(M, N, K) || !element_type_ok(type) || M > MOST_INPUTS || N > MOST_ROWS || K > 0x7FFFFF00) return 0;
     return linear_q4_workspace(M, N, K, type);
 }
 
@@ -2288,7 +2291,7 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
     if (st) return st;
     if ((st = q4_args_ok(N, K, group, scale_type))) return st;
     if (!element_type_ok(type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", type);
-    if (M > 0x7FFFFF00) return fail(CAKE_HIP_ERR_RANGE, "%d rows of x", M);   // padded to whole bands in 32-bit arithmetic
+    if (M > MOST_INPUTS) return fail(CAKE_HIP_ERR_RANGE, "%d rows of x (%d at most)", M, MOST_INPUTS);
     if (M == 0 || N == 0) return CAKE_HIP_OK;
     if (!y || (K > 0 && (!x || !q))) return fail(CAKE_HIP_ERR_ARG, "NULL operand");
     if ((st = ensure_init())) return st;
@@ -2362,9 +2365,8 @@ static int orthogonalize_scales(int steps, double c0, double c1, double c2, Orth
 static int orthogonalize_dims_ok(int batch, int rows, int cols)
 {
     if (batch < 0 || rows < 0 || cols < 0) return fail(CAKE_HIP_ERR_ARG, "negative dimension");
-    // sides are padded to whole blocks in 32-bit arithmetic
-    if (!fits_int((double)rows * cols) || rows > 0x7FFFFF00 || cols > 0x7FFFFF00)
-        return fail(CAKE_HIP_ERR_RANGE, "matrix of %dx%d exceeds 2^31 elements", rows, cols);
+    if (!fits_int((double)rows * cols) || rows > MOST_ROWS || cols > MOST_ROWS)
+        return fail(CAKE_HIP_ERR_RANGE, "matrix of %dx%d exceeds 2^31 elements or a side of 2^30", rows, cols);
     if (batch > 65535) return fail(CAKE_HIP_ERR_RANGE, "batch of %d matrices (65535 at most)", batch);
     return CAKE_HIP_OK;
 }

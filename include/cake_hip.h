@@ -410,7 +410,7 @@ enum { CAKE_HIP_F32 = 0, CAKE_HIP_F16 = 1, CAKE_HIP_BF16 = 2 };
 
 /* A weight matrix v[N][K] in 4 bits: code c[n][k] in 0..15 stands for (c - z) * s with one scale s and
  * one zero point z for each run of `group` columns of a row (group 32, 64 or 128; the last run of a row
- * may be short).  Scales and zero points are kept in scale_type; with_zeros == 0 keeps no zero points
+ * may be short); N stays below 2^30.  Scales and zero points are kept in scale_type; with_zeros == 0 keeps no zero points
  * and stands for z = 8.  The packed form is the library's own: cake_hip_q4_size bytes (0 for
  * arguments it does not take), 16-byte aligned, codes in the order the matrix pipe takes them, scales and
  * zero points behind; the same packed weights serve x of every type.  It has no counterpart
@@ -445,7 +445,7 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
 /* y[M][N] = x[M][K] . v[N][K]^T (+ bias[N] on every row when bias != NULL); x, bias and y are of `type`.
  * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and
  * zero points are applied to a run's sums in fp32, and y is rounded once.  The order of the sums depends
- * on the sizes, types and groups alone.  An infinity in x may come out as NaN in that row of y.  K == 0
+ * on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
  * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 16 rows of
  * x, 5 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
  * streams, two captured graphs) need workspaces of their own. */
@@ -461,7 +461,7 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
  * allowed).  With coefficients such as 3.4445, -4.7750, 2.0315 and 5 steps every singular value of g moves
  * close to 1, which is how the Muon optimiser treats the gradient of a weight matrix
  * (grad_w of cake_hip_linear_backward).
- * steps >= 1.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
+ * Sides stay below 2^30; steps >= 1.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
  * count as they are, the result is rounded once).  Singular values start in 0..1; coefficients whose
  * polynomial takes them beyond 1000 within `steps` are refused (CAKE_HIP_ERR_ARG).  x is kept to
  * 2^-23 of each value and no finer than 2^-39 (for the coefficients above), so a g whose

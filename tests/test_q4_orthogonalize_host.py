@@ -141,3 +141,14 @@ def test_torch_layer_refusals():
     with pytest.raises(ValueError):
         tl.cake_muon([torch.nn.Parameter(torch.zeros(5))])
     assert tl.orthogonalize(torch.zeros(0, 5)).shape == (0, 5)
+
+
+def test_sides_beyond_a_launch_are_refused():
+    """What would take 2^32 threads or more never reaches a launch."""
+    lib = cake.load()
+    b = _buf().ctypes.data
+    assert lib.cake_hip_q4_size(0x3FFFFF01, 1, 32, F32, 0) == 0 and lib.cake_hip_q4_size(0x3FFFFF00, 1, 32, F32, 0) > 0
+    assert lib.cake_hip_q4_pack(b, b, None, b, 0x3FFFFF01, 1, 32, F32, None, None) == _lib.ERR_RANGE
+    assert lib.cake_hip_linear_q4_forward(b, b, None, b, F32, 0x1FFFFF01, 1, 1, 32, F32, 0, None, None, None) == _lib.ERR_RANGE
+    assert lib.cake_hip_linear_q4_workspace(0x1FFFFF01, 1, 1, F32) == 0 < lib.cake_hip_linear_q4_workspace(0x1FFFFF00, 1, 1, F32)
+    assert _orth(rows=1, cols=0x3FFFFF01) == _lib.ERR_RANGE and _orth(rows=0x3FFFFF01, cols=1) == _lib.ERR_RANGE
