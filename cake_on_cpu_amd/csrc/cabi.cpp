@@ -2384,7 +2384,7 @@ int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int ro
     int st = orthogonalize_dims_ok(batch, rows, cols);
     if (st) return st;
     if (!element_type_ok(type)) return fail(CAKE_HIP_ERR_ARG, "unknown element type %d", type);
-    if (steps < 1) return fail(CAKE_HIP_ERR_ARG, "%d steps", steps);
+    if (steps < 1 || steps > 1000) return fail(CAKE_HIP_ERR_ARG, "%d steps (1 to 1000)", steps);   // one launch may run them all
     if (!(eps >= 0) || std::isinf(eps)) return fail(CAKE_HIP_ERR_ARG, "eps %g", eps);
     OrthogonalizeScales scales;
     if ((st = orthogonalize_scales(steps, c0, c1, c2, &scales))) return st;

@@ -461,7 +461,7 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
  * allowed).  With coefficients such as 3.4445, -4.7750, 2.0315 and 5 steps every singular value of g moves
  * close to 1, which is how the Muon optimiser treats the gradient of a weight matrix
  * (grad_w of cake_hip_linear_backward).
- * Sides stay below 2^30; steps >= 1.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
+ * Sides stay below 2^30; 1 to 1000 steps.  The norm is summed in fp64, the products to fp32 accuracy for every type (inputs
  * count as they are, the result is rounded once).  Singular values start in 0..1; coefficients whose
  * polynomial takes them beyond 1000 within `steps` are refused (CAKE_HIP_ERR_ARG).  x is kept to
  * 2^-23 of each value and no finer than 2^-39 (for the coefficients above), so a g whose

@@ -152,3 +152,9 @@ def test_sides_beyond_a_launch_are_refused():
     assert lib.cake_hip_linear_q4_forward(b, b, None, b, F32, 0x1FFFFF01, 1, 1, 32, F32, 0, None, None, None) == _lib.ERR_RANGE
     assert lib.cake_hip_linear_q4_workspace(0x1FFFFF01, 1, 1, F32) == 0 < lib.cake_hip_linear_q4_workspace(0x1FFFFF00, 1, 1, F32)
     assert _orth(rows=1, cols=0x3FFFFF01) == _lib.ERR_RANGE and _orth(rows=0x3FFFFF01, cols=1) == _lib.ERR_RANGE
+
+
+def test_steps_without_end_are_refused():
+    """A small matrix takes all its steps in one launch, which has to end."""
+    assert _orth(steps=1001) == _lib.ERR_ARG and _orth(steps=0x7FFFFFFF) == _lib.ERR_ARG
+    assert b"steps" in cake.load().cake_hip_last_error()
