@@ -553,16 +553,22 @@ class Q4Weight:
     __slots__ = ("data", "N", "K", "group", "scale_type", "with_zeros")
 
     def __init__(self, data, N, K, group, scale_type, with_zeros):
+        _any_ptr(data, "packed weights")
+        _need(data, _q4_bytes(N, K, group, scale_type, with_zeros), "packed weights")
         self.data, self.N, self.K, self.group = data, N, K, group
         self.scale_type, self.with_zeros = scale_type, bool(with_zeros)
 
 
-def q4_size(N, K, group=128, scale_dtype="float32", zeros=False) -> int:
-    """Bytes of the packed form."""
-    n = load().cake_hip_q4_size(N, K, group, element_type(scale_dtype), int(zeros))
-    if n == 0 and N > 0 and K > 0:
+def _q4_bytes(N, K, group, scale_type, zeros) -> int:
+    n = load().cake_hip_q4_size(N, K, group, scale_type, bool(zeros))
+    if n == 0 and N != 0 and K != 0:
         raise CakeHipError(_lib.ERR_ARG, "q4_size", load().cake_hip_last_error().decode())
     return n
+
+
+def q4_size(N, K, group=128, scale_dtype="float32", zeros=False) -> int:
+    """Bytes of the packed form."""
+    return _q4_bytes(N, K, group, element_type(scale_dtype), zeros)
 
 
 def _bytes_like(ref, n):
@@ -577,8 +583,6 @@ def _bytes_like(ref, n):
 
 def q4_of(data, N, K, group, scale_dtype, zeros) -> Q4Weight:
     """Packed bytes that an earlier q4_pack or q4_quantize made, with what they were made for."""
-    _any_ptr(data, "packed weights")
-    _need(data, q4_size(N, K, group, scale_dtype, zeros), "packed weights")
     return Q4Weight(data, N, K, group, element_type(scale_dtype), zeros)
 
 

@@ -135,8 +135,16 @@ def dequantize_q4(q, dtype=torch.float32):
     return w
 
 
-def _forward_q4(x, q, bias):
-    """x and bias contiguous, on the weights' device, checked by the caller"""
+def _forward_q4(input, q, bias):
+    if input.dim() != 2 or input.size(1) != q.K:
+        raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
+    if not q.data.is_contiguous():
+        raise TypeError("forward_q4: packed weights must be contiguous")
+    if bias is not None and (tuple(bias.shape) != (q.N,) or bias.dtype != input.dtype):
+        raise ValueError(f"forward_q4: bias {tuple(bias.shape)} of {bias.dtype} does not match {q.N} outputs of {input.dtype}")
+    if input.device != q.data.device or (bias is not None and bias.device != input.device):
+        raise ValueError(f"forward_q4: input on {input.device}, weights on {q.data.device}")
+    x, bias = input.contiguous(), None if bias is None else bias.contiguous()
     M = x.size(0)
     y = x.new_empty((M, q.N))
     if not x.is_cuda:
@@ -161,7 +169,7 @@ class cake_linear_q4_function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, data, q, bias):
         ctx.q, ctx.dtype = q, data.dtype
-        return _forward_q4(data.detach().contiguous(), q, None if bias is None else bias.detach().contiguous())
+        return _forward_q4(data.detach(), q, None if bias is None else bias.detach())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -178,17 +186,9 @@ class cake_linear_q4_function(torch.autograd.Function):
 def forward_q4(input, q, bias=None):
     """output[M][N] = input[M][K] . v[N][K]^T (+ bias) with v in 4 bits (pack_q4, quantize_q4).  input is float32,
     float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias."""
-    if input.dim() != 2 or input.size(1) != q.K:
-        raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
-    if not q.data.is_contiguous():
-        raise TypeError("forward_q4: packed weights must be contiguous")
-    if bias is not None and (tuple(bias.shape) != (q.N,) or bias.dtype != input.dtype):
-        raise ValueError(f"forward_q4: bias {tuple(bias.shape)} of {bias.dtype} does not match {q.N} outputs of {input.dtype}")
-    if input.device != q.data.device or (bias is not None and bias.device != input.device):
-        raise ValueError(f"forward_q4: input on {input.device}, weights on {q.data.device}")
     if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
         return cake_linear_q4_function.apply(input, q, bias)
-    return _forward_q4(input.contiguous(), q, None if bias is None else bias.contiguous())
+    return _forward_q4(input, q, bias)
 
 
 class cake_linear_q4(nn.Module):

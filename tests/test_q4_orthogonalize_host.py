@@ -158,3 +158,22 @@ def test_steps_without_end_are_refused():
     """A small matrix takes all its steps in one launch, which has to end."""
     assert _orth(steps=1001) == _lib.ERR_ARG and _orth(steps=0x7FFFFFFF) == _lib.ERR_ARG
     assert b"steps" in cake.load().cake_hip_last_error()
+
+
+def test_packed_weights_hold_what_they_say():
+    """Sizes are checked where packed weights are made and where the layer's function is applied by itself."""
+    torch = pytest.importorskip("torch")
+    from cake_on_cpu_amd import torch_linear as tl
+    held = torch.zeros(cake.q4_size(8, 8, 32), dtype=torch.uint8)
+    for bad in ((held[:-1], 8, 8, 32, F32, False), (held, 17, 8, 32, F32, False), (held, 8, 8, 32, F32, True)):
+        with pytest.raises(ValueError):
+            cake.Q4Weight(*bad)
+    for bad in ((held, 8, 8, 48, F32, False), (held, 8, 8, 32, 9, False), (held, -8, 8, 32, F32, False)):
+        with pytest.raises(cake.CakeHipError):
+            cake.Q4Weight(*bad)
+    with pytest.raises(TypeError):
+        cake.Q4Weight(held.float(), 8, 8, 32, F32, False)
+    q = cake.Q4Weight(held, 8, 8, 32, F32, False)
+    for x, bias in ((torch.zeros(2, 7), None), (torch.zeros(2, 8), torch.zeros(7))):
+        with pytest.raises(ValueError):
+            tl.cake_linear_q4_function.apply(x.requires_grad_(), q, bias)
