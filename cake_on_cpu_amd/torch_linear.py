@@ -169,12 +169,13 @@ class cake_linear_q4_function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, data, q, bias):
         ctx.q, ctx.dtype = q, data.dtype
+        ctx.save_for_backward(q.data)   # to notice a change before the backward pass reads it
         return _forward_q4(data.detach(), q, None if bias is None else bias.detach())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        q, M = ctx.q, grad_output.size(0)
+        _, q, M = ctx.saved_tensors, ctx.q, grad_output.size(0)
         g = grad_output.detach().float().contiguous()
         gx = torch.empty((M, q.K), dtype=torch.float32, device=g.device) if ctx.needs_input_grad[0] else None
         gb = torch.empty((q.N,), dtype=torch.float32, device=g.device) if ctx.needs_input_grad[2] else None
@@ -211,8 +212,19 @@ class cake_linear_q4(nn.Module):
     def weight_q4(self):
         return api.Q4Weight(self.packed, self.output_features, self.input_features, self.group, self.scale_type, self.with_zeros)
 
+    def get_extra_state(self):
+        """What the packed bytes were made for, a tensor as everything else that is stored."""
+        return torch.tensor([self.output_features, self.input_features, self.group, self.scale_type, int(self.with_zeros)])
+
+    def set_extra_state(self, state):
+        if state.tolist() != self.get_extra_state().tolist():
+            raise ValueError(f"cake_linear_q4: stored weights are {state.tolist()} (outputs, inputs, group, scale type, zeros), "
+                             f"this layer's {self.get_extra_state().tolist()}")
+
     def forward(self, data):
-        flat = data.reshape(-1, self.input_features)
+        if data.dim() == 0 or data.size(-1) != self.input_features:
+            raise ValueError(f"cake_linear_q4: input {tuple(data.shape)} does not match {self.input_features} columns of weights")
+        flat = data.reshape(data.shape[:-1].numel(), self.input_features)
         bias = None if self.bias is None else self.bias.to(data.dtype)
         return forward_q4(flat, self.weight_q4, bias).reshape(*data.shape[:-1], self.output_features)
 

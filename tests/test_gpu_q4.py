@@ -331,3 +331,55 @@ def test_an_input_of_tiny_values():
         want = x.double() @ v64.t()
         tol = (16 * 2 + 48) * 2.0 ** -24 * (x.double().abs() @ mass.t())
         assert bool(((tl.forward_q4(x.cuda(), q).double().cpu() - want).abs() <= tol).all()), rows
+
+
+def test_layer_without_tokens_or_columns():
+    held = tl.cake_linear_q4.of(tl.cake_linear(300, 130).cuda(), group=64, zeros=True)
+    assert held(torch.zeros(2, 0, 300, device="cuda")).shape == (2, 0, 130)
+    assert held(torch.zeros(300, device="cuda")).shape == (130,)
+    none = tl.cake_linear_q4(cake.q4_of(torch.zeros(0, dtype=torch.uint8, device="cuda"), 5, 0, 32, torch.float32, False), torch.arange(5.0, device="cuda"))
+    for shape in ((2, 3, 0), (40, 0)):
+        assert torch.equal(none(torch.zeros(shape, device="cuda")), torch.arange(5.0, device="cuda").expand(*shape[:-1], 5))
+
+
+def test_weights_changed_before_the_backward_pass_are_noticed():
+    q = tl.quantize_q4(torch.randn(32, 128, device="cuda"), 64)
+    x = torch.randn(3, 128, device="cuda", requires_grad=True)
+    y = tl.forward_q4(x, q)
+    q.data.zero_()
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
+
+
+def test_captured_forward_and_backward_replay():
+    """The whole step in one graph, replayed on changed inputs with eager work of the same sizes in between."""
+    M, N, K = 40, 96, 320
+    q = tl.quantize_q4(torch.randn(N, K, generator=torch.Generator().manual_seed(1)).cuda(), 64, True)
+    x = torch.zeros(M, K, device="cuda", requires_grad=True)
+    gy = torch.zeros(M, N, device="cuda")
+
+    def eager(xs, g):
+        leaf = xs.clone().requires_grad_()
+        y = tl.forward_q4(leaf, q)
+        return y.detach(), torch.autograd.grad(y, leaf, g)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(tl.forward_q4(x, q), x, gy)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = tl.forward_q4(x, q)
+        gx, = torch.autograd.grad(y, x, gy)
+    for i in range(4):
+        gen = torch.Generator().manual_seed(10 + i)
+        with torch.no_grad():
+            x.copy_(torch.randn(M, K, generator=gen))
+            gy.copy_(torch.randn(M, N, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_g = eager(x.detach(), gy)
+        assert torch.equal(y, want) and torch.equal(gx, want_g), i

@@ -177,3 +177,22 @@ def test_packed_weights_hold_what_they_say():
     for x, bias in ((torch.zeros(2, 7), None), (torch.zeros(2, 8), torch.zeros(7))):
         with pytest.raises(ValueError):
             tl.cake_linear_q4_function.apply(x.requires_grad_(), q, bias)
+
+
+def test_layer_refuses_what_is_not_its_own():
+    """Stored bytes of another group size, type of scales or kind are other weights, also where their number is the same."""
+    torch = pytest.importorskip("torch")
+    from cake_on_cpu_amd import torch_linear as tl
+
+    def layer(N=16, K=128, group=32, dtype=torch.bfloat16, zeros=False):
+        return tl.cake_linear_q4(cake.q4_of(torch.zeros(cake.q4_size(N, K, group, dtype, zeros), dtype=torch.uint8), N, K, group, dtype, zeros))
+
+    stored = layer().state_dict()
+    assert all(isinstance(v, torch.Tensor) for v in stored.values())
+    layer().load_state_dict(stored)
+    for other in (layer(dtype=torch.float16), layer(group=64), layer(N=15)):
+        with pytest.raises((ValueError, RuntimeError)):
+            other.load_state_dict(stored)
+    for x in (torch.zeros(3, 64), torch.zeros(3, 256), torch.zeros(128, 3), torch.tensor(1.0)):
+        with pytest.raises(ValueError):
+            layer()(x)
