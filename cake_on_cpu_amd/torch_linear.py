@@ -111,6 +111,8 @@ def pack_q4(codes, scales, zeros, in_features, group=128):
     half of a byte), scales and zeros (or None: 8) [N][ceil(K / group)]."""
     if codes.dim() != 2 or codes.size(1) != (in_features + 1) // 2:
         raise ValueError(f"pack_q4: codes {tuple(codes.shape)} do not hold {in_features} columns")
+    if group not in (32, 64, 128):
+        raise ValueError(f"pack_q4: group of {group} (32, 64 or 128)")
     want = (codes.size(0), -(-in_features // group))
     for t, what in ((scales, "scales"), (zeros, "zeros")):
         if t is not None and tuple(t.shape) != want:
@@ -263,10 +265,16 @@ class cake_muon(torch.optim.Optimizer):
                  eps=1e-7):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps))
-        for group in self.param_groups:
-            for w in group["params"]:
-                if w.dim() != 2:
+
+    def add_param_group(self, param_group):
+        params = param_group["params"]
+        if not isinstance(params, set):   # (which the base class refuses: it has no order)
+            params = [params] if isinstance(params, torch.Tensor) else list(params)
+            for w in params:
+                w = w[1] if isinstance(w, tuple) else w   # (name, parameter)
+                if isinstance(w, torch.Tensor) and w.dim() != 2:
                     raise ValueError(f"cake_muon: parameter {tuple(w.shape)} is no matrix")
+        super().add_param_group({**param_group, "params": params})
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -196,3 +196,26 @@ def test_layer_refuses_what_is_not_its_own():
     for x in (torch.zeros(3, 64), torch.zeros(3, 256), torch.zeros(128, 3), torch.tensor(1.0)):
         with pytest.raises(ValueError):
             layer()(x)
+
+
+def test_optimiser_takes_matrices_alone_also_later():
+    torch = pytest.importorskip("torch")
+    from cake_on_cpu_amd import torch_linear as tl
+    w = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = tl.cake_muon(iter([w]))
+    for shape in ((5,), (2, 3, 4)):
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": torch.nn.Parameter(torch.zeros(shape))})
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(shape))], "lr": 0.1})
+    opt.add_param_group({"params": (v for v in [torch.nn.Parameter(torch.zeros(4, 4))]), "lr": 0.5})
+    assert [len(g["params"]) for g in opt.param_groups] == [1, 1] and opt.param_groups[1]["lr"] == 0.5
+    for bad in ([3], {torch.nn.Parameter(torch.zeros(2, 2))}):
+        with pytest.raises(TypeError):
+            tl.cake_muon(bad) if isinstance(bad, list) else opt.add_param_group({"params": bad})
+    with pytest.raises(ValueError):
+        tl.cake_muon([("bias", torch.nn.Parameter(torch.zeros(2)))])
+    assert len(tl.cake_muon(torch.nn.Linear(3, 4, bias=False).named_parameters()).param_groups[0]["params"]) == 1
+    for group in (0, 48):
+        with pytest.raises(ValueError):
+            tl.pack_q4(torch.zeros(8, 4, dtype=torch.uint8), torch.zeros(8, 1), None, 8, group)
