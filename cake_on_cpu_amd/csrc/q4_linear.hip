@@ -45,38 +45,41 @@ struct StreamArgs {
 // its 8 columns of its row for each of the four steps, straight in operand order.  32-bit x: the wave
 // fetches two columns a lane, cuts them into pieces and passes them through LDS of its own; no
 // other wave takes part, so nothing waits at a barrier.
-template <int TYPE, int REGS>
+template <int TYPE, int REGS, int MT>
 struct BlockOfX {
     typedef typename Element<TYPE>::T T;
-    uintx4 step[4];
+    uintx4 step[MT][4];
     __device__ __forceinline__ void fetch(const T* x, int M, int K, int block, int lane, int my_row)
     {
         const int k = block * 128 + (lane >> 4) * 8;
         const bool whole = block * 128 + 128 <= K;   // the same for the whole wave
 #pragma unroll
-        for (int i = 0; i < 4; ++i) step[i] = uintx4{0, 0, 0, 0};
-        if (my_row < M) {
-            const T* at = x + (size_t)my_row * K + k;
-            if (whole) {
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) __builtin_memcpy(&step[i], at + 32 * i, 16);
-            } else {
+            for (int i = 0; i < 4; ++i) step[mt][i] = uintx4{0, 0, 0, 0};
+            if (my_row + 16 * mt < M) {
+                const T* at = x + (size_t)(my_row + 16 * mt) * K + k;
+                if (whole) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    T v[8];
-                    load_eight<TYPE>(at + 32 * i, K - k - 32 * i, v);
-                    step[i] = piece_of<TYPE>(v, 0);
+                    for (int i = 0; i < 4; ++i) __builtin_memcpy(&step[mt][i], at + 32 * i, 16);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        T v[8];
+                        load_eight<TYPE>(at + 32 * i, K - k - 32 * i, v);
+                        step[mt][i] = piece_of<TYPE>(v, 0);
+                    }
                 }
             }
         }
     }
     static constexpr int TOKENS = 0;
     __device__ __forceinline__ void to_lds(unsigned char*, int) const {}
-    __device__ __forceinline__ uintx4 operand(int i, const unsigned char*, bool) const { return step[i]; }
+    __device__ __forceinline__ uintx4 operand(int mt, int i, const unsigned char*, bool) const { return step[mt][i]; }
 };
-template <int REGS>
-struct BlockOfX<CAKE_HIP_F32, REGS> {
-    static constexpr int TOKENS = REGS == 1 ? 1 : 5;   // whose pieces fill 4 or 16 rows
+template <int REGS, int MT>
+struct BlockOfX<CAKE_HIP_F32, REGS, MT> {
+    static constexpr int TOKENS = REGS == 1 ? 1 : 5 * MT;   // whose pieces fill 4, 16 or 32 rows
     float v[TOKENS][2];
     __device__ __forceinline__ void fetch(const float* x, int M, int K, int block, int lane, int)
     {
@@ -112,22 +115,22 @@ struct BlockOfX<CAKE_HIP_F32, REGS> {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __device__ __forceinline__ uintx4 operand(int i, const unsigned char* mine_row, bool real) const
+    __device__ __forceinline__ uintx4 operand(int mt, int i, const unsigned char* mine_row, bool real) const
     {
-        const uintx4 got = *reinterpret_cast<const uintx4*>(mine_row + i * TOKENS * 3 * 64);
+        const uintx4 got = *reinterpret_cast<const uintx4*>(mine_row + (real ? mt * 1024 : 0) + i * TOKENS * 3 * 64);
         return real ? got : uintx4{0, 0, 0, 0};
     }
 };
 
-// Few rows of x (up to 16 of pieces): the codes are read once, straight into the registers of the
+// Few rows of x (up to 16 MT of pieces): the codes are read once, straight into the registers of the
 // wave that multiplies them.  A workgroup owns NT tiles of 16 rows of v; its waves share the blocks of
 // 128 columns out among them in turn, DEPTH turns in flight each, and add their sums up through LDS
 // in a fixed order.
 // Row r of pieces is A's row 4 (r & 3) + (r >> 2), so that the first four rows come out in the four lanes'
 // first result register and REGS registers cover 4 REGS rows: with one token the scale costs two
 // operations per group instead of eight.
-template <int TYPE, int GPB, bool WIDE, int REGS, int NT>
-__global__ __launch_bounds__(1024 / NT) void linear_q4_stream_kernel(StreamArgs a)
+template <int TYPE, int GPB, bool WIDE, int REGS, int NT, int MT>
+__global__ __launch_bounds__(NT * MT == 1 ? 1024 : 512) void linear_q4_stream_kernel(StreamArgs a)
 {
     typedef typename Element<TYPE>::T T;
     constexpr int PIECES = pieces_of<TYPE>();
@@ -142,17 +145,16 @@ __global__ __launch_bounds__(1024 / NT) void linear_q4_stream_kernel(StreamArgs 
 
     // this lane's row of the A operand, and the place of its columns in the wave's own LDS (32-bit x)
     const int my_row = (col & 3) * 4 + (col >> 2);
-    const bool real = my_row < rows;
-    constexpr int OWN = BlockOfX<TYPE, REGS>::TOKENS * 3 * 256;
+    constexpr int OWN = BlockOfX<TYPE, REGS, MT>::TOKENS * 3 * 256;
     unsigned char* mine = lds + wave * OWN;
-    const unsigned char* mine_row = mine + (real ? my_row * 64 + quad * 16 : 0);
+    const unsigned char* mine_row = mine + (my_row < rows ? my_row * 64 + quad * 16 : 0);
 
     struct Held {
         uintx4 code[NT];
         GroupValues<GPB, WIDE> s[NT], z[NT];
     } held[DEPTH];
-    constexpr int X_SETS = GPB == 4 ? 2 : DEPTH;   // four groups' scales leave registers for the next turn's x only
-    BlockOfX<TYPE, REGS> x[X_SETS];
+    constexpr int X_SETS = GPB == 4 || MT == 2 ? 2 : DEPTH;   // four groups' scales or twice the rows leave registers for the next turn's x only
+    BlockOfX<TYPE, REGS, MT> x[X_SETS];
     // addresses are scalars that move on by the waves' number of blocks, and a lane's place in a block
     constexpr int SCALE_BYTES = 16 * GPB * (WIDE ? 4 : 2);
     const bool half = a.lay.scale_type == CAKE_HIP_F16;
@@ -183,32 +185,48 @@ __global__ __launch_bounds__(1024 / NT) void linear_q4_stream_kernel(StreamArgs 
         if (block < blocks) x[set].fetch(static_cast<const T*>(a.x), a.M, K, block, lane, my_row);
     };
 
-    floatx4 acc[NT];
+    floatx4 acc[MT][NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[nt] = floatx4{0, 0, 0, 0};
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = floatx4{0, 0, 0, 0};
     uintx4 ones;
 #pragma unroll
     for (int i = 0; i < 4; ++i) ones[i] = Codes<TYPE>::ONES;
 
-    auto multiply = [&](const Held& h, const BlockOfX<TYPE, REGS>& bx) {
+    auto multiply = [&](const Held& h, const BlockOfX<TYPE, REGS, MT>& bx) {
         bx.to_lds(mine, lane);
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
-            floatx4 p[NT], sum = floatx4{0, 0, 0, 0};
+            floatx4 p[MT][NT], sum[MT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) p[nt] = floatx4{0, 0, 0, 0};
+            for (int mt = 0; mt < MT; ++mt) {
+                sum[mt] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) p[mt][nt] = floatx4{0, 0, 0, 0};
+            }
 #pragma unroll
             for (int i = g * SG; i < (g + 1) * SG; ++i) {
-                const uintx4 xa = bx.operand(i, mine_row, real);
-                sum = Codes<TYPE>::mfma(xa, ones, sum);
+                uintx4 xa[MT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) p[nt] = Codes<TYPE>::mfma(xa, unpack_codes<TYPE>(h.code[nt][i]), p[nt]);
+                for (int mt = 0; mt < MT; ++mt) {
+                    xa[mt] = bx.operand(mt, i, mine_row, my_row + 16 * mt < rows);
+                    sum[mt] = Codes<TYPE>::mfma(xa[mt], ones, sum[mt]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uintx4 codes = unpack_codes<TYPE>(h.code[nt][i]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) p[mt][nt] = Codes<TYPE>::mfma(xa[mt], codes, p[mt][nt]);
+                }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float s = h.s[nt].at(g, half), z = a.with_zeros ? h.z[nt].at(g, half) : 8.f;
 #pragma unroll
-                for (int r = 0; r < REGS; ++r) acc[nt][r] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[r], p[nt][r]), acc[nt][r]);
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < REGS; ++r) acc[mt][nt][r] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[mt][r], p[mt][nt][r]), acc[mt][nt][r]);
             }
             if (GPB == 4) __builtin_amdgcn_sched_barrier(0);   // all groups' codes unpacked at once have no room in registers
         }
@@ -235,12 +253,14 @@ __global__ __launch_bounds__(1024 / NT) void linear_q4_stream_kernel(StreamArgs 
     float* red = reinterpret_cast<float*>(lds);
     constexpr int WIDTH = NT * 16;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int r = 0; r < REGS; ++r) {
-            const int row = r * 4 + quad;
-            if (row < rows) red[(wave * rows + row) * WIDTH + nt * 16 + col] = acc[nt][r];
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < REGS; ++r) {
+                const int row = mt * 16 + r * 4 + quad;
+                if (row < rows) red[(wave * rows + row) * WIDTH + nt * 16 + col] = acc[mt][nt][r];
+            }
     __syncthreads();
     for (int i = threadIdx.x; i < a.M * WIDTH; i += blockDim.x) {
         const int m = i / WIDTH, c = i - m * WIDTH, n = tile0 * 16 + c;
@@ -260,10 +280,10 @@ hipError_t stream_launch(const StreamArgs& a, hipStream_t stream)
     const int rows = a.M * pieces_of<TYPE>();
     // two tiles a workgroup share x and its column sums, as soon as that leaves a workgroup for every compute unit
     const int nt = a.lay.tiles >= 512 ? 2 : 1;
-    int waves = nt == 1 ? 16 : 8;
+    int waves = nt == 1 && rows <= 16 ? 16 : 8;
     while (waves > 1 && waves / 2 >= a.lay.blocks) waves /= 2;
     // the waves' sums; before that, of a 32-bit x, their blocks of pieces
-    const size_t own = TYPE == CAKE_HIP_F32 ? (rows <= 4 ? 3 : 15) * 256 : 0;
+    const size_t own = TYPE == CAKE_HIP_F32 ? (rows <= 4 ? 3 : rows <= 16 ? 15 : 30) * 256 : 0;
     const size_t lds = waves * std::max((size_t)rows * nt * 64, own);
     const dim3 grid((a.lay.tiles + nt - 1) / nt), block(64 * waves);
     auto run = [&](auto kernel) {
@@ -272,27 +292,31 @@ hipError_t stream_launch(const StreamArgs& a, hipStream_t stream)
     };
     auto of_width = [&](auto wide) {
         constexpr bool W = decltype(wide)::value;
-        if (rows <= 4) return nt == 1 ? run(&linear_q4_stream_kernel<TYPE, GPB, W, 1, 1>) : run(&linear_q4_stream_kernel<TYPE, GPB, W, 1, 2>);
-        return nt == 1 ? run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 1>) : run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 2>);
+        if (rows <= 4) return nt == 1 ? run(&linear_q4_stream_kernel<TYPE, GPB, W, 1, 1, 1>) : run(&linear_q4_stream_kernel<TYPE, GPB, W, 1, 2, 1>);
+        if (rows <= 16) return nt == 1 ? run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 1, 1>) : run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 2, 1>);
+        return nt == 1 ? run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 1, 2>) : run(&linear_q4_stream_kernel<TYPE, GPB, W, 4, 2, 2>);
     };
     return a.lay.scale_type == CAKE_HIP_F32 ? of_width(std::true_type()) : of_width(std::false_type());
 }
 
-// what fits one tile of 16 rows of pieces is streamed
-bool streams(int M, int type) { return M <= (type == CAKE_HIP_F32 ? 5 : 16); }
+// What fits two tiles of 16 rows of pieces is streamed: one launch instead of three (17 rows of 4096 x 4096 9.8 us,
+// in a band 15.9; of 14336 x 4096 in groups of 32 21 and 34; 10 of fp32 12 and 20).  Every workgroup reads all of x
+// itself, though, and with more than 24 rows of many columns that costs more (32 rows of 4096 x 14336 30 and
+// 27, of 16384 x 16384 71 and 63, but of 4096 x 4096 12 and 16).
+bool streams(int M, int K, int type) { return type == CAKE_HIP_F32 ? M <= 10 : M <= 24 || (M <= 32 && K <= 8192); }
 
 }  // namespace
 
 size_t linear_q4_workspace(int M, int N, int K, int type)
 {
-    return M == 0 || N == 0 || streams(M, type) ? 0 : linear_q4_bands_workspace(M, N, K, type);
+    return M == 0 || N == 0 || streams(M, K, type) ? 0 : linear_q4_bands_workspace(M, N, K, type);
 }
 
 hipError_t launch_linear_q4(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
                             bool with_zeros, void* workspace, hipStream_t stream)
 {
     hipError_t e = hipSuccess;
-    if (streams(M, type)) {
+    if (streams(M, lay.K, type)) {
         StreamArgs a{};
         a.x = x;
         a.q = static_cast<const unsigned char*>(q);

@@ -446,8 +446,8 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
  * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and
  * zero points are applied to a run's sums in fp32, and y is rounded once.  The order of the sums depends
  * on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
- * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 16 rows of
- * x, 5 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
+ * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 24 rows of
+ * x, 10 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
  * streams, two captured graphs) need workspaces of their own. */
 size_t cake_hip_linear_q4_workspace(int M, int N, int K, int type);
 int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, void* y, int type, int M, int N, int K,

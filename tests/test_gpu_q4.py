@@ -383,3 +383,25 @@ def test_captured_forward_and_backward_replay():
         torch.cuda.synchronize()
         want, want_g = eager(x.detach(), gy)
         assert torch.equal(y, want) and torch.equal(gx, want_g), i
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_rows_of_every_number_and_many_outputs(kind):
+    """More outputs than 512 tiles, an odd number of tiles, and either side of every number of rows and columns at
+    which the kernel changes."""
+    N = 8200
+    for K, group, zeros, rows in ((1111, 32, True, (1, 3, 4, 5, 6, 9, 10, 11, 16, 17, 24, 25, 31, 32, 33)), (300, 128, False, (2, 6, 10, 17, 32)),
+                                  (640, 64, True, (5, 8, 20, 29))):
+        packed, s, z, v64, mass = _weights(N, K, group, zeros, torch.float32 if group == 32 else torch.bfloat16, K)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+        for M in rows:
+            print(f"linear_q4 M={M} N={N} K={K} {kind} group={group}", flush=True)
+            x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(TYPES[kind]).cuda()
+            _check(tl.forward_q4(x, q), x, v64, mass, None, K)
+    for K in (8192, 8193):
+        packed, s, z, v64, mass = _weights(40, K, 64, False, torch.float16, K)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None, K, 64)
+        for M in (10, 24, 25, 32):
+            print(f"linear_q4 M={M} K={K} {kind}", flush=True)
+            x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(TYPES[kind]).cuda()
+            _check(tl.forward_q4(x, q), x, v64, mass, None, K)
