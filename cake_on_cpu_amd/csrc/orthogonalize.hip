@@ -176,6 +176,15 @@ __device__ __forceinline__ void tile_of(int id, int tiles_i, int& ti, int& tj)
     }
 }
 
+// Workgroups are dealt out to the eight dies in turn, each with an L2 of its own.  Where k is sliced they are
+// numbered so that a die's are consecutive and it reads an eighth of the operands, not all of them (a of 1024 x 4096
+// in 7 slices 22 to 20 us); without slices either order takes the same time.
+__device__ __forceinline__ int die_order(int id, int all)
+{
+    const int die = id & 7, each = all >> 3;
+    return die * each + min(die, all & 7) + (id >> 3);
+}
+
 // a of the lanes where `upper` is not set and b of the lanes where it is, exchanged for the partner's other one
 template <int PARTNER>
 __device__ __forceinline__ void swap_across(unsigned& a, unsigned& b, bool upper)
@@ -295,7 +304,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void pair_gemm_kernel(PairGemm g)
     const int wi = wave / WJ, wj = wave % WJ;
 
     int ti, tj;
-    const int slice = blockIdx.x / g.tiles, tile = blockIdx.x - slice * g.tiles;
+    const int id = g.slices > 1 ? die_order(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+    const int slice = id / g.tiles, tile = id - slice * g.tiles;
     tile_of<MODE>(tile, g.tiles_i, ti, tj);
     const int k0 = (int)((long long)g.kb * slice / g.slices), k1 = (int)((long long)g.kb * (slice + 1) / g.slices);
     const _Float16* p = g.p + blockIdx.z * g.p_stride;
@@ -380,7 +390,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void pair_gemm_kernel(PairGemm g)
     }
 
     if (g.partial) {
-        float* to = g.partial + (((size_t)blockIdx.z * gridDim.x + blockIdx.x) * (BI * BJ)) * 256 + lane * 4;
+        float* to = g.partial + (((size_t)blockIdx.z * gridDim.x + id) * (BI * BJ)) * 256 + lane * 4;
 #pragma unroll
         for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -419,13 +429,13 @@ __global__ __launch_bounds__(256) void join_slices_kernel(PairGemm g, int tile_b
 }
 
 // The four tiles, and what a stage of 32 columns and a tile's beginning and end take in microseconds
-// (measured on sides of 1024 to 4096): `alone` with one workgroup on a compute unit, `full`
+// (measured on sides of 256 to 4096): `alone` with one workgroup on a compute unit, `full`
 // with as many as fit.
 struct TileCost {
     int blocks, resident;
     float alone, full;
 };
-constexpr TileCost TILES[] = {{4, 4, 0.42f, 1.1f}, {8, 2, 0.75f, 1.42f}, {12, 1, 1.42f, 1.42f}, {16, 1, 2.35f, 2.35f}};
+constexpr TileCost TILES[] = {{4, 4, 0.34f, 1.1f}, {8, 2, 0.75f, 1.42f}, {12, 1, 1.42f, 1.42f}, {16, 1, 2.35f, 2.35f}};
 // The device's compute units; a number of this file, so that the size of the workspace and the order of
 // the sums follow from the sizes alone.
 constexpr int CUS = 256;
@@ -452,10 +462,11 @@ TileChoice choose_tile(int ib, int jb, int kb, bool symmetric, int batch)
             const float groups = tiles * s;
             if (s > 1 && groups > CUS * t.resident) break;
             const float rounds = ceilf(groups / (CUS * t.resident));
-            const float stage = groups <= CUS ? t.alone : t.full;
+            const float beside = fminf(ceilf(groups / CUS), (float)t.resident) - 1;   // others on the same compute unit
+            const float stage = beside > 0 ? t.alone + (t.full - t.alone) * beside / (float)(t.resident - 1) : t.alone;
             float us = 3.f + rounds * (stage * ((kb + s - 1) / s) + 3.f);
-            // partial sums out and back at about 3 TB/s, and a launch
-            if (s > 1) us += 4.f + groups * t.blocks * t.blocks * 2048 / 3e6f;
+            // partial sums out and back at about 6 TB/s, and a launch
+            if (s > 1) us += 5.f + 0.15f * s + groups * t.blocks * t.blocks * 2048 / 6e6f;
             if (us < least) {
                 least = us;
                 best = {w, s};
