@@ -44,6 +44,15 @@ __device__ __forceinline__ size_t pair_at(int row, int col, int row_blocks)
     return ((size_t)(col >> 5) * row_blocks + (row >> 4)) * (2 * BLOCK) + ((row & 15) + ((col >> 3) & 3) * 16) * 8 + (col & 7);
 }
 
+// The same for the first element of the 16 x 16 half of a block at blocks (bi, bj) of 16, the same for a whole wave;
+// behind it lies (row, col) at col / 8 * 128 + row * 8 + col % 8.
+__device__ __forceinline__ size_t half_at(int bi, int bj, int row_blocks)
+{
+    return ((size_t)(bj >> 1) * row_blocks + bi) * (2 * BLOCK) + (bj & 1) * (BLOCK / 2);
+}
+// Where a lane finds rows 4 (lane >> 4) + 0..3 of column lane & 15 of a half that is kept turned: 4 consecutive halves
+__device__ __forceinline__ unsigned turned_lane(unsigned lane) { return (lane >> 5) * 128 + (lane & 15) * 8 + (lane >> 4 & 1) * 4; }
+
 // The carried x: blocks of 16 x 16 floats, four a lane as a product's results come out of the matrix pipe.
 __device__ __forceinline__ size_t carried_at(int bi, int bj, int row_blocks) { return ((size_t)bj * row_blocks + bi) * 256; }
 
@@ -198,7 +207,7 @@ __device__ __forceinline__ void swap_across(unsigned& a, unsigned& b, bool upper
 // [column][rows]: 8 bytes a lane and whole lines a wave.
 __device__ __forceinline__ void store_along(_Float16* out, int bi, int bj, int row_blocks, f16x4 hi, f16x4 lo, int lane)
 {
-    _Float16* to = out + pair_at(bj * 16 + (lane & 15), bi * 16 + (lane >> 4) * 4, row_blocks);
+    _Float16* to = out + half_at(bj, bi, row_blocks) + turned_lane(lane);
     *reinterpret_cast<f16x4*>(to) = hi;
     *reinterpret_cast<f16x4*>(to + BLOCK) = lo;
 }
@@ -224,7 +233,7 @@ __device__ __forceinline__ void store_across(_Float16* out, int bi, int bj, int 
         h[r] = (w[2 * r] & 0xFFFFu) | w[2 * r + 1] << 16;
         l[r] = w[2 * r] >> 16 | (w[2 * r + 1] & 0xFFFF0000u);
     }
-    _Float16* to = out + pair_at(bi * 16 + (lane >> 4) * 4 + (lane & 3), bj * 16 + (lane & 12), row_blocks);
+    _Float16* to = out + half_at(bi, bj, row_blocks) + ((unsigned)(lane >> 3 & 1) * 128 + ((lane >> 4) * 4 + (lane & 3)) * 8 + (lane & 4));
     *reinterpret_cast<uintx2*>(to) = h;
     *reinterpret_cast<uintx2*>(to + BLOCK) = l;
 }
@@ -247,7 +256,7 @@ __device__ __forceinline__ void finish_block(const PairGemm& g, int z, int bi, i
     const int row = bi * 16 + (lane >> 4) * 4, c = bj * 16 + (lane & 15);
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] *= g.unscale;
-    const size_t turned = pair_at(c, row, g.jb);   // (column, rows): 4 consecutive halves
+    const size_t turned = half_at(bj, bi, g.jb) + turned_lane(lane);
     if (MODE >= APPLY) {
         floatx4* x = reinterpret_cast<floatx4*>(g.carried + z * (g.out_stride / 2) + carried_at(bi, bj, g.ib) + lane * 4);
         floatx4 was;
@@ -414,7 +423,7 @@ __global__ __launch_bounds__(256) void join_slices_kernel(PairGemm g, int tile_b
 {
     const int lane = threadIdx.x & 63;
     const int per_tile = tile_blocks * tile_blocks;
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = unit / per_tile, block = unit - tile * per_tile;
     if (tile >= g.tiles) return;
     int ti, tj;
@@ -661,7 +670,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
             const int bi = a_bi[t], bj = a_bj[t];
             if (wave + t * waves < squares) {
                 const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, as + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.mb / 2);
-                const _Float16* a = as + pair_at(bj * 16 + (lane & 15), bi * 16 + (lane >> 4) * 4, s.mb);
+                const _Float16* a = as + half_at(bj, bi, s.mb) + turned_lane(lane);
                 const f16x4 ah = *reinterpret_cast<const f16x4*>(a), al = *reinterpret_cast<const f16x4*>(a + BLOCK);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) square[t][r] = s.c2 * (v[r] * down_aa) + s.c1 * (((float)ah[r] + (float)al[r]) * down_a);
