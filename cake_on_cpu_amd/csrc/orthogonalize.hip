@@ -531,11 +531,14 @@ size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
 
 // ---- small matrices ------------------------------------------------------------------------
 // One workgroup per matrix and one launch: a matrix whose pairs and whose square's pairs fit the LDS of a
-// compute unit together (sides up to 128 x 160, 64 x 560, 32 x 1200).  x stays in registers in fp32, in
+// compute unit together (sides up to 128 x 160, 64 x 544, 32 x 1200).  x stays in registers in fp32, in
 // blocks as they come out of the matrix pipe; its pairs are written to LDS along its columns for
 // a = x x^T and then, over them, along its rows for b x.  Launches of a product each cost 5 to 6 us
 // at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 45 us in one.
-enum { SMALL_WAVES = 16, SMALL_X_BLOCKS = 10, SMALL_A_BLOCKS = 3 };   // blocks a wave holds of x and of the square
+// The products are bound by what LDS delivers, so a wave takes units of 2 x 2 blocks, half the operands a
+// block, wherever there is more than a block or two for every wave.
+enum { SMALL_WAVES = 16 };
+constexpr int small_units(int x_side, int a_side) { return x_side == 2 && a_side == 1 ? 3 : 2; }   // of x in a wave; of the square it holds one
 
 struct SmallArgs {
     const void* g;
@@ -547,10 +550,10 @@ struct SmallArgs {
     float up_x, up_a, up_b;
 };
 
-// The sum over kb column blocks of one block's product.  The next operands are on their way while these
-// are multiplied, and the small products have a sum of their own, so that a matrix instruction waits
-// for one before it rather than for two.
-__device__ __forceinline__ floatx4 pair_product(const _Float16* p, const _Float16* q, int step_p, int step_q, int kb)
+// The sums over kb column blocks of a unit's products.  For a single block the next operands are on their way while
+// these are multiplied, and the small products have a sum of their own, so that a matrix instruction
+// waits for one before it rather than for two.
+__device__ __forceinline__ void unit_product(const _Float16* p, const _Float16* q, int step_p, int step_q, int kb, floatx4 (&sum)[1][1])
 {
     floatx4 acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
     f16x8 ph = *reinterpret_cast<const f16x8*>(p), pl = *reinterpret_cast<const f16x8*>(p + BLOCK);
@@ -571,46 +574,85 @@ __device__ __forceinline__ floatx4 pair_product(const _Float16* p, const _Float1
     low = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, low, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
     low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, low, 0, 0, 0);
-    return acc + low;
+    sum[0][0] = acc + low;
+}
+__device__ __forceinline__ void unit_product(const _Float16* p, const _Float16* q, int step_p, int step_q, int kb, floatx4 (&sum)[2][2])
+{
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) sum[a][b] = floatx4{0, 0, 0, 0};
+    for (int k = 0; k < kb; ++k) {
+        f16x8 ph[2], pl[2], qh[2], ql[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ph[a] = *reinterpret_cast<const f16x8*>(p + a * 2 * BLOCK);
+            pl[a] = *reinterpret_cast<const f16x8*>(p + a * 2 * BLOCK + BLOCK);
+            qh[a] = *reinterpret_cast<const f16x8*>(q + a * 2 * BLOCK);
+            ql[a] = *reinterpret_cast<const f16x8*>(q + a * 2 * BLOCK + BLOCK);
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[a], qh[b], sum[a][b], 0, 0, 0);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], ql[b], sum[a][b], 0, 0, 0);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], qh[b], sum[a][b], 0, 0, 0);
+        p += step_p;
+        q += step_q;
+    }
 }
 
+// XS, AS: sides of a unit of x and of the square.
+template <int XS, int AS>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallArgs s)
 {
     extern __shared__ __align__(16) _Float16 stage[];
     __shared__ double norms[SMALL_WAVES];
+    constexpr int UNITS = small_units(XS, AS);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     _Float16* const xs = stage;                          // pairs of x, then of its transpose
     _Float16* const as = stage + s.mb * s.nb * BLOCK;    // pairs of a, then of b
-    const int blocks = s.mb * s.nb, squares = s.mb * (s.mb + 1) / 2;
+    const int rows = s.mb / XS, units = rows * (s.nb / XS), squares = (s.mb / AS) * (s.mb / AS + 1) / 2;
     const size_t base = (size_t)blockIdx.x * s.m * s.n;
     auto index = [&](int i, int j) { return base + (s.tall ? (size_t)j * s.m + i : (size_t)i * s.n + j); };
 
-    // this wave's blocks of x and of the square
-    int x_bi[SMALL_X_BLOCKS], x_bj[SMALL_X_BLOCKS], a_bi[SMALL_A_BLOCKS], a_bj[SMALL_A_BLOCKS];
+    // this wave's blocks of x, and those of the square
+    int x_bi[UNITS], x_bj[UNITS], a_bi, a_bj;
 #pragma unroll
-    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
-        x_bi[t] = (wave + t * waves) % s.mb;
-        x_bj[t] = (wave + t * waves) / s.mb;
+    for (int t = 0; t < UNITS; ++t) {
+        x_bi[t] = (wave + t * waves) % rows * XS;
+        x_bj[t] = (wave + t * waves) / rows * XS;
     }
-#pragma unroll
-    for (int t = 0; t < SMALL_A_BLOCKS; ++t) tile_of<GRAM>(wave + t * waves, 0, a_bi[t], a_bj[t]);
+    tile_of<GRAM>(wave, 0, a_bi, a_bj);
+    a_bi *= AS;
+    a_bj *= AS;
 
-    floatx4 x[SMALL_X_BLOCKS];
+    floatx4 x[UNITS][XS][XS];
     double sum = 0;
 #pragma unroll
-    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
-        const int block = wave + t * waves;
-        x[t] = floatx4{0, 0, 0, 0};
-        if (block < blocks) {
-            const int i = x_bi[t] * 16 + (lane >> 4) * 4, j = x_bj[t] * 16 + (lane & 15);
+    for (int t = 0; t < UNITS; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (i + r < s.m && j < s.n) {
-                    x[t][r] = load_as_float(s.g, index(i + r, j), s.type);
-                    sum += (double)x[t][r] * (double)x[t][r];
+        for (int a = 0; a < XS; ++a)
+#pragma unroll
+            for (int b = 0; b < XS; ++b) {
+                x[t][a][b] = floatx4{0, 0, 0, 0};
+                if (wave + t * waves < units) {
+                    const int i = (x_bi[t] + a) * 16 + (lane >> 4) * 4, j = (x_bj[t] + b) * 16 + (lane & 15);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i + r < s.m && j < s.n) {
+                            const float v = load_as_float(s.g, index(i + r, j), s.type);
+                            x[t][a][b][r] = v;
+                            sum += (double)v * (double)v;
+                        }
                 }
-        }
-    }
+            }
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) norms[wave] = sum;
     __syncthreads();
@@ -619,94 +661,121 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small_matrices_kernel(SmallA
     const double length = sqrt(sum) + s.eps;
     const double by = length == 0 ? 0 : 1.0 / length;   // zeros stay zeros also without an eps
 #pragma unroll
-    for (int t = 0; t < SMALL_X_BLOCKS; ++t)
+    for (int t = 0; t < UNITS; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[t][r] = (float)((double)x[t][r] * by);
+        for (int a = 0; a < XS; ++a)
+#pragma unroll
+            for (int b = 0; b < XS; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[t][a][b][r] = (float)((double)x[t][a][b][r] * by);
 
     const float down_aa = 1.f / (s.up_a * s.up_a), down_xx = 1.f / (s.up_x * s.up_x), down_bx = 1.f / (s.up_b * s.up_x), down_a = 1.f / s.up_a;
     auto store_x = [&](bool along) {
 #pragma unroll
-        for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
-            const int block = wave + t * waves;
-            if (block < blocks) {
-                f16x4 hi, lo;
-                split4(x[t], s.up_x, hi, lo);
-                if (along) store_along(xs, x_bi[t], x_bj[t], s.nb, hi, lo, lane);
-                else store_across(xs, x_bi[t], x_bj[t], s.mb, hi, lo, lane);
+        for (int t = 0; t < UNITS; ++t)
+            if (wave + t * waves < units) {
+#pragma unroll
+                for (int a = 0; a < XS; ++a)
+#pragma unroll
+                    for (int b = 0; b < XS; ++b) {
+                        f16x4 hi, lo;
+                        split4(x[t][a][b], s.up_x, hi, lo);
+                        if (along) store_along(xs, x_bi[t] + a, x_bj[t] + b, s.nb, hi, lo, lane);
+                        else store_across(xs, x_bi[t] + a, x_bj[t] + b, s.mb, hi, lo, lane);
+                    }
             }
-        }
     };
+    const int step_a = s.mb * 2 * BLOCK;
     for (int step = 0; step < s.steps; ++step) {
         store_x(false);
         __syncthreads();
-        floatx4 square[SMALL_A_BLOCKS];
+        floatx4 square[AS][AS];
         auto store_squares = [&](float up) {
+            if (wave < squares) {
 #pragma unroll
-            for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-                const int bi = a_bi[t], bj = a_bj[t];
-                if (wave + t * waves < squares) {
-                    f16x4 hi, lo;
-                    split4(square[t], up, hi, lo);
-                    store_along(as, bi, bj, s.mb, hi, lo, lane);
-                    if (bi != bj) store_across(as, bi, bj, s.mb, hi, lo, lane);
-                }
+                for (int a = 0; a < AS; ++a)
+#pragma unroll
+                    for (int b = 0; b < AS; ++b) {
+                        const int bi = a_bi + a, bj = a_bj + b;
+                        if (bi > bj) continue;   // the lower half of a unit on the diagonal comes from its upper one
+                        f16x4 hi, lo;
+                        split4(square[a][b], up, hi, lo);
+                        store_along(as, bi, bj, s.mb, hi, lo, lane);
+                        if (bi != bj) store_across(as, bi, bj, s.mb, hi, lo, lane);
+                    }
             }
         };
-        const int step_a = s.mb * 2 * BLOCK;
+        if (wave < squares) {
+            unit_product(xs + a_bi * 2 * BLOCK + lane * 8, xs + a_bj * 2 * BLOCK + lane * 8, step_a, step_a, s.nb / 2, square);
 #pragma unroll
-        for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-            const int bi = a_bi[t], bj = a_bj[t];
-            if (wave + t * waves < squares) {
-                const floatx4 v = pair_product(xs + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.nb / 2);
+            for (int a = 0; a < AS; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) square[t][r] = v[r] * down_xx;
-            }
+                for (int b = 0; b < AS; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) square[a][b][r] *= down_xx;
         }
         store_squares(s.up_a);   // the first time into memory that nobody reads, then behind the barrier after b x
         __syncthreads();
         store_x(true);           // a is complete: nobody reads x along its columns any more
+        if (wave < squares) {
+            unit_product(as + a_bi * 2 * BLOCK + lane * 8, as + a_bj * 2 * BLOCK + lane * 8, step_a, step_a, s.mb / 2, square);
 #pragma unroll
-        for (int t = 0; t < SMALL_A_BLOCKS; ++t) {
-            const int bi = a_bi[t], bj = a_bj[t];
-            if (wave + t * waves < squares) {
-                const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, as + bj * 2 * BLOCK + lane * 8, step_a, step_a, s.mb / 2);
-                const _Float16* a = as + half_at(bj, bi, s.mb) + turned_lane(lane);
-                const f16x4 ah = *reinterpret_cast<const f16x4*>(a), al = *reinterpret_cast<const f16x4*>(a + BLOCK);
+            for (int a = 0; a < AS; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) square[t][r] = s.c2 * (v[r] * down_aa) + s.c1 * (((float)ah[r] + (float)al[r]) * down_a);
-            }
+                for (int b = 0; b < AS; ++b) {
+                    const _Float16* at = as + half_at(a_bj + b, a_bi + a, s.mb) + turned_lane(lane);
+                    const f16x4 ah = *reinterpret_cast<const f16x4*>(at), al = *reinterpret_cast<const f16x4*>(at + BLOCK);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        square[a][b][r] = s.c2 * (square[a][b][r] * down_aa) + s.c1 * (((float)ah[r] + (float)al[r]) * down_a);
+                }
         }
         __syncthreads();
         store_squares(s.up_b);
         __syncthreads();
 #pragma unroll
-        for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
-            const int block = wave + t * waves;
-            if (block < blocks) {
-                const int bi = x_bi[t], bj = x_bj[t];
-                const floatx4 v = pair_product(as + bi * 2 * BLOCK + lane * 8, xs + bj * 2 * BLOCK + lane * 8, step_a, s.nb * 2 * BLOCK, s.mb / 2);
+        for (int t = 0; t < UNITS; ++t)
+            if (wave + t * waves < units) {
+                floatx4 v[XS][XS];
+                unit_product(as + x_bi[t] * 2 * BLOCK + lane * 8, xs + x_bj[t] * 2 * BLOCK + lane * 8, step_a, s.nb * 2 * BLOCK, s.mb / 2, v);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[t][r] = __builtin_fmaf(s.c0, x[t][r], v[r] * down_bx);
+                for (int a = 0; a < XS; ++a)
+#pragma unroll
+                    for (int b = 0; b < XS; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[t][a][b][r] = __builtin_fmaf(s.c0, x[t][a][b][r], v[a][b][r] * down_bx);
             }
-        }
         __syncthreads();
     }
 #pragma unroll
-    for (int t = 0; t < SMALL_X_BLOCKS; ++t) {
-        const int block = wave + t * waves;
-        if (block < blocks) {
-            const int i = x_bi[t] * 16 + (lane >> 4) * 4, j = x_bj[t] * 16 + (lane & 15);
+    for (int t = 0; t < UNITS; ++t)
+        if (wave + t * waves < units) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (i + r < s.m && j < s.n) store_from_float(s.out, index(i + r, j), s.type, x[t][r]);
+            for (int a = 0; a < XS; ++a)
+#pragma unroll
+                for (int b = 0; b < XS; ++b) {
+                    const int i = (x_bi[t] + a) * 16 + (lane >> 4) * 4, j = (x_bj[t] + b) * 16 + (lane & 15);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i + r < s.m && j < s.n) store_from_float(s.out, index(i + r, j), s.type, x[t][a][b][r]);
+                }
         }
-    }
+}
+
+// Sides of the units: single blocks where they are no more than two a wave (the square: one).
+int small_x_side(int mb, int nb) { return mb * nb <= 2 * SMALL_WAVES ? 1 : 2; }
+int small_a_side(int mb) { return mb <= 4 ? 1 : 2; }
+int small_x_units(int mb, int nb) { return mb * nb / (small_x_side(mb, nb) * small_x_side(mb, nb)); }
+int small_a_units(int mb)
+{
+    const int side = mb / small_a_side(mb);
+    return side * (side + 1) / 2;
 }
 
 // a block of 16 x 32 pairs is 2 KB: mb nb / 2 of them for x, mb mb / 2 for the square, 1 KB left for the norm
 bool small_fits(int mb, int nb)
 {
-    return mb * nb + mb * mb <= 159 && mb * nb <= SMALL_WAVES * SMALL_X_BLOCKS && mb * (mb + 1) / 2 <= SMALL_WAVES * SMALL_A_BLOCKS;
+    return mb * nb + mb * mb <= 159 && small_x_units(mb, nb) <= SMALL_WAVES * small_units(small_x_side(mb, nb), small_a_side(mb)) && small_a_units(mb) <= SMALL_WAVES;
 }
 
 }  // namespace
@@ -743,13 +812,14 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     if (small_fits(l.mb, l.nb)) {
         SmallArgs a{g, out, type, l.m, l.n, l.mb, l.nb, steps, tall, (float)c0, (float)c1, (float)c2, eps, up_x, up_a, up_b};
         const size_t lds = (size_t)(l.mb * l.nb + l.mb * l.mb) * 1024;
+        const int waves = std::min<int>(SMALL_WAVES, std::max(small_x_units(l.mb, l.nb), small_a_units(l.mb)));
+        auto kernel = small_a_side(l.mb) == 2 ? &small_matrices_kernel<2, 2>
+                                              : small_x_side(l.mb, l.nb) == 2 ? &small_matrices_kernel<2, 1> : &small_matrices_kernel<1, 1>;
         if (lds > 63 * 1024) {
-            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&small_matrices_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e != hipSuccess) return e;
         }
-        // a wave per block of x at least while there are more waves than that; squares never need more than the same
-        const int waves = std::min<int>(SMALL_WAVES, l.mb * l.nb);
-        small_matrices_kernel<<<batch, 64 * waves, lds, stream>>>(a);
+        kernel<<<batch, 64 * waves, lds, stream>>>(a);
         return hipGetLastError();
     }
     char* ws = static_cast<char*>(workspace);

@@ -282,3 +282,17 @@ def test_a_row_of_more_than_2_to_the_25_columns():
         assert float((out - along * unit).abs().max()) <= 5 * 10 * 3 * 2.0 ** -23 * 1.3 * float(unit.abs().max())
         del g, out, unit
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(64, 544), (64, 545), (30, 1216), (1217, 30), (50, 270), (20, 520), (33, 97), (97, 129), (96, 320), (90, 321), (128, 160), (110, 161)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_orthogonalize_at_the_ends_of_one_launch(shape):
+    """The largest matrices that one workgroup takes, the smallest that it does not, and every kind of units between."""
+    for kind in TYPES:
+        g = _gradient(*shape, seed=sum(shape)).to(TYPES[kind])
+        print(f"orthogonalize {shape} {kind}", flush=True)
+        _check(tl.orthogonalize(g.cuda()), g, 5)
+    three = torch.stack([_gradient(*shape, seed=s) for s in range(3)])
+    out = tl.orthogonalize(three.cuda())
+    for i in range(3):
+        _check(out[i], three[i], 5)
