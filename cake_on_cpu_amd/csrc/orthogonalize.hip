@@ -591,6 +591,7 @@ __device__ __forceinline__ void unit_product(const _Float16* p, const _Float16* 
             qh[a] = *reinterpret_cast<const f16x8*>(q + a * 2 * BLOCK);
             ql[a] = *reinterpret_cast<const f16x8*>(q + a * 2 * BLOCK + BLOCK);
         }
+        __builtin_amdgcn_sched_barrier(0);   // one wait for all eight, not one for each
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
