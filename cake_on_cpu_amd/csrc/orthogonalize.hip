@@ -534,7 +534,7 @@ size_t slice_floats(int ib, int jb, int kb, bool symmetric, int batch)
 // compute unit together (sides up to 128 x 160, 64 x 544, 32 x 1200).  x stays in registers in fp32, in
 // blocks as they come out of the matrix pipe; its pairs are written to LDS along its columns for
 // a = x x^T and then, over them, along its rows for b x.  Launches of a product each cost 5 to 6 us
-// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 45 us in one.
+// at these sizes whatever they do: 16 matrices of 96 x 130 took 98 us in 17 launches, 42 us in one.
 // The products are bound by what LDS delivers, so a wave takes units of 2 x 2 blocks, half the operands a
 // block, wherever there is more than a block or two for every wave.
 enum { SMALL_WAVES = 16 };
