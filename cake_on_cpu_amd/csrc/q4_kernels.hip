@@ -234,17 +234,12 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const unsigned char* __res
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = reorder_nibbles(w[i]);
     *reinterpret_cast<uintx4*>(q + unit * 1024 + lane * 16) = out;
-    if (quad == 0) {
-        const int groups = (lay.K + 128 / GPB - 1) / (128 / GPB);
-#pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-            const size_t at = (unit * 16 + lane) * GPB + g;
-            const int gk = block * GPB + g;
-            const bool real = row < lay.N && gk < groups;
-            const size_t in = (size_t)row * groups + gk;
-            store_from_float(q + lay.scales_at, at, lay.scale_type, real ? load_as_float(scales, in, lay.scale_type) : 0.f);
-            if (zeros) store_from_float(q + lay.zeros_at, at, lay.scale_type, real ? load_as_float(zeros, in, lay.scale_type) : 0.f);
-        }
+    if (lane < 16 * GPB) {   // a lane per scale, in the order they are kept
+        const int groups = (lay.K + 128 / GPB - 1) / (128 / GPB), n = tile * 16 + lane / GPB, gk = block * GPB + lane % GPB;
+        const bool real = n < lay.N && gk < groups;
+        const size_t at = unit * 16 * GPB + lane, in = (size_t)n * groups + gk;
+        store_from_float(q + lay.scales_at, at, lay.scale_type, real ? load_as_float(scales, in, lay.scale_type) : 0.f);
+        if (zeros) store_from_float(q + lay.zeros_at, at, lay.scale_type, real ? load_as_float(zeros, in, lay.scale_type) : 0.f);
     }
 }
 
