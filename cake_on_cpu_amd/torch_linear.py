@@ -219,9 +219,14 @@ class cake_linear_q4(nn.Module):
         return torch.tensor([self.output_features, self.input_features, self.group, self.scale_type, int(self.with_zeros)])
 
     def set_extra_state(self, state):
-        if state.tolist() != self.get_extra_state().tolist():
+        pass   # compared before anything is copied
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        state = state_dict.get(prefix + "_extra_state")
+        if state is not None and state.tolist() != self.get_extra_state().tolist():
             raise ValueError(f"cake_linear_q4: stored weights are {state.tolist()} (outputs, inputs, group, scale type, zeros), "
                              f"this layer's {self.get_extra_state().tolist()}")
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def forward(self, data):
         if data.dim() == 0 or data.size(-1) != self.input_features:

@@ -219,3 +219,22 @@ def test_optimiser_takes_matrices_alone_also_later():
     for group in (0, 48):
         with pytest.raises(ValueError):
             tl.pack_q4(torch.zeros(8, 4, dtype=torch.uint8), torch.zeros(8, 1), None, 8, group)
+
+
+def test_a_refused_load_changes_nothing():
+    torch = pytest.importorskip("torch")
+    from cake_on_cpu_amd import torch_linear as tl
+
+    def layer(fill, dtype):
+        data = torch.full((cake.q4_size(16, 128, 32, dtype, False),), fill, dtype=torch.uint8)
+        return tl.cake_linear_q4(cake.q4_of(data, 16, 128, 32, dtype, False), torch.zeros(16))
+
+    held, stored = layer(1, torch.bfloat16), layer(2, torch.float16).state_dict()
+    with pytest.raises(ValueError):
+        held.load_state_dict(stored)
+    assert bool((held.packed == 1).all())
+    model, other = torch.nn.Sequential(layer(1, torch.float16)), torch.nn.Sequential(layer(2, torch.float16))
+    model.load_state_dict(other.state_dict())
+    assert bool((model[0].packed == 2).all())
+    with pytest.raises(RuntimeError):       # strict: what the bytes were made for has to be there
+        model.load_state_dict({k: v for k, v in other.state_dict().items() if "extra" not in k})
