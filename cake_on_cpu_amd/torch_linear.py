@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import api
 
@@ -137,6 +138,15 @@ def dequantize_q4(q, dtype=torch.float32):
     return w
 
 
+_is_tracing = torch._C._is_tracing   # (a lookup less: one token is bound by the host's call)
+
+
+def _watched():
+    """Whether torch has to see an operator although nothing needs its gradient: a trace records what becomes of
+    tensors and not what is written through a pointer, and a dual tensor's tangent is not to be lost in silence."""
+    return _is_tracing() or forward_ad._current_level >= 0
+
+
 def _forward_q4(input, q, bias):
     if input.dim() != 2 or input.size(1) != q.K:
         raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
@@ -169,9 +179,12 @@ class cake_linear_q4_function(torch.autograd.Function):
     """Gradients of the layer for its input and bias; the packed weights are constants."""
 
     @staticmethod
-    def forward(ctx, data, q, bias):
+    def forward(ctx, data, q, bias, packed=None):
+        """packed: q's bytes once more, as a tensor that a trace connects with where they come from."""
+        if packed is not None and packed is not q.data:   # replayed
+            q = api.Q4Weight(packed, q.N, q.K, q.group, q.scale_type, q.with_zeros)
         ctx.q, ctx.dtype = q, data.dtype
-        ctx.save_for_backward(q.data)   # to notice a change before the backward pass reads it
+        ctx.save_for_backward(q.data if packed is None else packed)   # to notice a change before the backward pass reads it
         return _forward_q4(data.detach(), q, None if bias is None else bias.detach())
 
     @staticmethod
@@ -183,14 +196,15 @@ class cake_linear_q4_function(torch.autograd.Function):
         gb = torch.empty((q.N,), dtype=torch.float32, device=g.device) if ctx.needs_input_grad[2] else None
         w = dequantize_q4(q) if gx is not None else None
         api.linear_backward(g, None, w, gx, None, gb, M, q.N, q.K, timed=not g.is_cuda)
-        return None if gx is None else gx.to(ctx.dtype), None, None if gb is None else gb.to(ctx.dtype)
+        return None if gx is None else gx.to(ctx.dtype), None, None if gb is None else gb.to(ctx.dtype), None
 
 
 def forward_q4(input, q, bias=None):
     """output[M][N] = input[M][K] . v[N][K]^T (+ bias) with v in 4 bits (pack_q4, quantize_q4).  input is float32,
-    float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias."""
-    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
-        return cake_linear_q4_function.apply(input, q, bias)
+    float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias (reverse
+    mode; a tangent of forward mode is refused)."""
+    if (torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad))) or _watched():
+        return cake_linear_q4_function.apply(input, q, bias, q.data)
     return _forward_q4(input, q, bias)
 
 
@@ -231,7 +245,7 @@ class cake_linear_q4(nn.Module):
     def forward(self, data):
         if data.dim() == 0 or data.size(-1) != self.input_features:
             raise ValueError(f"cake_linear_q4: input {tuple(data.shape)} does not match {self.input_features} columns of weights")
-        flat = data.reshape(data.shape[:-1].numel(), self.input_features)
+        flat = data.flatten(0, -2) if data.dim() > 1 else data.unsqueeze(0)   # (no number of rows that a trace would keep)
         bias = None if self.bias is None else self.bias.to(data.dtype)
         return forward_q4(flat, self.weight_q4, bias).reshape(*data.shape[:-1], self.output_features)
 
