@@ -107,9 +107,38 @@ class cake_linear(nn.Module):
 # ---- the layer with 4-bit weights -------------------------------------------------------
 
 
+_is_tracing = torch._C._is_tracing   # (a lookup less: one token is bound by the host's call)
+
+
+def _watched():
+    """Whether torch has to see an operator although nothing needs its gradient: a trace records what becomes of
+    tensors and not what is written through a pointer, and a dual tensor's tangent is not to be lost in silence."""
+    return _is_tracing() or forward_ad._current_level >= 0
+
+
+class _recorded_function(torch.autograd.Function):
+    """compute(tensor) as one operation of a trace; it has no gradient."""
+
+    @staticmethod
+    def forward(ctx, tensor, compute):
+        out = compute(tensor.detach())
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return None, None
+
+
+def _not_in_a_trace(what):
+    if _is_tracing():
+        raise RuntimeError(f"{what}: a trace cannot record what packs weights; pack them before it and trace the layer")
+
+
 def pack_q4(codes, scales, zeros, in_features, group=128):
     """Packed weights from an existing checkpoint's tensors: codes[N][(K + 1) // 2] (uint8, even columns in the low
     half of a byte), scales and zeros (or None: 8) [N][ceil(K / group)]."""
+    _not_in_a_trace("pack_q4")
     if codes.dim() != 2 or codes.size(1) != (in_features + 1) // 2:
         raise ValueError(f"pack_q4: codes {tuple(codes.shape)} do not hold {in_features} columns")
     if group not in (32, 64, 128):
@@ -126,6 +155,7 @@ def pack_q4(codes, scales, zeros, in_features, group=128):
 
 def quantize_q4(weight, group=128, zeros=False, scale_dtype=torch.bfloat16):
     """A weight matrix in 4 bits with one scale (and, with `zeros`, one zero point) for `group` columns of a row."""
+    _not_in_a_trace("quantize_q4")
     if weight.dim() != 2:
         raise ValueError(f"quantize_q4: weight {tuple(weight.shape)} is no matrix")
     return api.q4_quantize(weight.detach().contiguous(), *weight.shape, group=group, zeros=zeros, scale_dtype=scale_dtype)
@@ -133,18 +163,12 @@ def quantize_q4(weight, group=128, zeros=False, scale_dtype=torch.bfloat16):
 
 def dequantize_q4(q, dtype=torch.float32):
     """The values that packed weights stand for, as a tensor [N][K]."""
-    w = torch.empty((q.N, q.K), dtype=dtype, device=q.data.device)
-    api.q4_dequantize(q, w)
-    return w
+    def values(packed):
+        w = torch.empty((q.N, q.K), dtype=dtype, device=packed.device)
+        api.q4_dequantize(q if packed is q.data else api.Q4Weight(packed, q.N, q.K, q.group, q.scale_type, q.with_zeros), w)
+        return w
 
-
-_is_tracing = torch._C._is_tracing   # (a lookup less: one token is bound by the host's call)
-
-
-def _watched():
-    """Whether torch has to see an operator although nothing needs its gradient: a trace records what becomes of
-    tensors and not what is written through a pointer, and a dual tensor's tangent is not to be lost in silence."""
-    return _is_tracing() or forward_ad._current_level >= 0
+    return _recorded_function.apply(q.data, values) if _is_tracing() else values(q.data)
 
 
 def _forward_q4(input, q, bias):
@@ -262,8 +286,14 @@ def orthogonalize(grad, steps=5, coefficients=api.NEWTON_SCHULZ, eps=1e-7):
     matrices have their singular values moved close to 1.  Not differentiable."""
     if grad.dim() < 2:
         raise ValueError(f"orthogonalize: {tuple(grad.shape)} is no matrix")
+    if _is_tracing():
+        return _recorded_function.apply(grad, lambda g: _orthogonalize(g, steps, coefficients, eps))
+    return _orthogonalize(grad.detach(), steps, coefficients, eps)
+
+
+def _orthogonalize(grad, steps, coefficients, eps):
     rows, cols = grad.shape[-2:]
-    g = grad.detach().contiguous()
+    g = grad.contiguous()
     out = torch.empty_like(g)
     if g.numel() == 0:
         return out

@@ -80,3 +80,36 @@ def test_a_traced_layer_computes(stand_in, bias, grad):
         traced.load_state_dict({**traced.state_dict(), "packed": _packed(7)})
         want = _layer(7, bias)
         assert torch.equal(traced(x), want(x))
+
+
+@pytest.fixture
+def stand_ins(monkeypatch, stand_in):
+    def dequantize(q, w, timed=False):
+        _at(w, q.N * q.K)[:] = int(q.data.flatten()[0])
+
+    def orthogonalize(g, out, batch, rows, cols, steps, coefficients, eps, workspace=None, timed=True):
+        _at(out, batch * rows * cols)[:] = _at(g, batch * rows * cols) * steps
+
+    monkeypatch.setattr(api, "q4_dequantize", dequantize)
+    monkeypatch.setattr(api, "orthogonalize", orthogonalize)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_traced_update_computes(stand_ins, grad):
+    """orthogonalize and dequantize_q4 are recorded as themselves; what packs weights is refused in a trace."""
+    gen = torch.Generator().manual_seed(2)
+    g = torch.randn(2, 4, 6, generator=gen, requires_grad=grad)
+    q = cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    update = torch.jit.trace(lambda v: tl.orthogonalize(v, steps=4), (g,), check_trace=False)
+    weights = torch.jit.trace(lambda v: v @ tl.dequantize_q4(q).t(), (torch.randn(2, K),), check_trace=False)
+    for _ in range(3):
+        g = torch.randn(2, 4, 6, generator=gen, requires_grad=grad)
+        keep = [torch.full(s, float("nan")) for s in ((2, 4, 6), (N, K)) for _ in range(8)]
+        del keep
+        out = update(g)
+        assert torch.equal(out, 4 * g.detach()) and not out.requires_grad and not tl.orthogonalize(g).requires_grad
+        x = torch.randn(2, K, generator=gen)
+        assert torch.equal(weights(x), x @ torch.full((K, N), 3.0))
+    for call in (lambda w: tl.dequantize_q4(tl.quantize_q4(w)), lambda s: tl.dequantize_q4(tl.pack_q4(torch.zeros(4, 8, dtype=torch.uint8), s[:, :1], None, 16))):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (torch.randn(4, 16),), check_trace=False)
