@@ -21,6 +21,8 @@ KERNEL_NAMES = {0: "macro-tile", 1: "matrix-vector", 2: "streaming, few rows", 3
                 4: "short K, tiles walked by resident workgroups",
                 5: "256 x 128 tiles walked by one resident workgroup per CU"}
 
+NULL_STREAM = 1   # as a stream argument the null stream on every context, where 0 is the context's own
+
 F32, F16, BF16 = range(3)   # element types of the 4-bit linear layer and of orthogonalize
 
 OK, ERR_ARG, ERR_NO_DEVICE, ERR_HIP, ERR_ALLOC, ERR_RANGE, ERR_ARCH = range(7)

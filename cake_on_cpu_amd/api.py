@@ -50,11 +50,13 @@ def _stream(*arrays) -> int:
 
 def _torch_stream(torch, device) -> int:
     """The handle of torch's current stream on `device`, without the stream object where this torch
-    has the short way (0.1 us instead of 1.7: a short kernel's call is bound by the host)."""
+    has the short way (0.1 us instead of 1.7: a short kernel's call is bound by the host).  The default stream's
+    is 0 in torch and has a name of its own here: a 0 would be the stream of the current context, which does not
+    wait for what torch has enqueued."""
     short = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if short is None or device.index is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return short(device.index)
+        return torch.cuda.current_stream(device).cuda_stream or _lib.NULL_STREAM
+    return short(device.index) or _lib.NULL_STREAM
 
 
 def _numel(a) -> int:
@@ -403,8 +405,8 @@ class Context:
     made while it is current do not share with the default context or with other contexts.
 
         with cake.Context() as ctx:          # current on this thread inside the block
-            cake.cake_sgemm(...)             # device operands: enqueued on ctx.stream unless torch's
-                                             # current stream is passed by the operands
+            cake.cake_sgemm(...)             # torch tensors on the GPU: on torch's current stream, host operands
+                                             # on ctx.stream
     """
 
     def __init__(self):

@@ -178,6 +178,7 @@ inline Context& cur() { return t_current_ctx ? *t_current_ctx : g_default_ctx; }
 // the stream argument of an entry point: NULL means the current context's own stream
 inline hipStream_t pick_stream(void* stream_)
 {
+    if (stream_ == CAKE_HIP_NULL_STREAM) return nullptr;
     return stream_ ? static_cast<hipStream_t>(stream_) : cur().own_stream;
 }
 

@@ -15,7 +15,8 @@
  * kernels ran on); staging copies are not part of it.
  *
  * Streams.  `stream` is a hipStream_t passed as void*; NULL is the default
- * stream.  With device operands and seconds == NULL a call only enqueues work.
+ * stream (of a context made by cake_hip_ctx_create: its own), CAKE_HIP_NULL_STREAM
+ * the null stream whatever the context.  With device operands and seconds == NULL a call only enqueues work.
  *
  * Every function returns CAKE_HIP_OK (0) or an error code; no function calls
  * exit().  cake_hip_last_error() gives the text of the last failure on the
@@ -146,10 +147,13 @@ const char* cake_hip_last_error(void);
  * makes a context for the device of the default one, with a non-blocking stream of its own.
  * cake_hip_ctx_set_current(ctx) makes it the calling thread's context (NULL: back to the default);
  * from then on a NULL `stream` argument means the context's own stream (cake_hip_ctx_stream), where
- * on the default context it means the HIP null stream.  cake_hip_ctx_destroy waits for the device
+ * on the default context it means the HIP null stream.  The own stream does not wait for work on the null
+ * stream; a caller whose operands are made there (the default stream of a framework, whose handle is 0)
+ * passes CAKE_HIP_NULL_STREAM.  cake_hip_ctx_destroy waits for the device
  * and frees the context's device memory, events and stream; a thread that still has it current
  * gets CAKE_HIP_ERR_ARG from its next call.  cake_hip_sgemm_noalloc on any context uses the
  * device's one scratch array. */
+#define CAKE_HIP_NULL_STREAM ((void*)1)   /* the value of hipStreamLegacy */
 typedef void* cake_hip_ctx_t;
 int cake_hip_ctx_create(cake_hip_ctx_t* out);
 int cake_hip_ctx_destroy(cake_hip_ctx_t ctx);

@@ -10,7 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import cake_on_cpu_amd as cake
-from cake_on_cpu_amd import api
+from cake_on_cpu_amd import _lib, api
 from cake_on_cpu_amd import torch_linear as tl
 
 pytestmark = pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
@@ -113,3 +113,20 @@ def test_a_traced_update_computes(stand_ins, grad):
     for call in (lambda w: tl.dequantize_q4(tl.quantize_q4(w)), lambda s: tl.dequantize_q4(tl.pack_q4(torch.zeros(4, 8, dtype=torch.uint8), s[:, :1], None, 16))):
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(call, (torch.randn(4, 16),), check_trace=False)
+
+
+def test_a_call_names_torchs_default_stream(monkeypatch):
+    """The handle of torch's default stream is 0, which the C entries take for the current context's own stream: a call
+    on tensors names the null stream instead, so that it runs behind the work that made them."""
+    class Torch:
+        class _C:
+            handle = 0
+            _cuda_getCurrentRawStream = staticmethod(lambda index: Torch._C.handle)
+
+        class cuda:
+            current_stream = staticmethod(lambda device: type("Stream", (), {"cuda_stream": Torch._C.handle}))
+
+    for device in (torch.device("cuda:0"), torch.device("cuda")):
+        for Torch._C.handle, want in ((0, _lib.NULL_STREAM), (0x1234, 0x1234)):
+            assert api._torch_stream(Torch, device) == want
+    assert _lib.NULL_STREAM != 0 and api._stream(np.zeros(1, np.float32), torch.zeros(1)) == 0   # host operands: the context's own
