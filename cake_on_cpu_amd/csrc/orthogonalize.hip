@@ -9,7 +9,7 @@
 // hi hi + hi lo + lo hi -- three matrix instructions where the fp32 ones, at a sixteenth of the rate,
 // would take the time of sixteen -- summed in 32 bits; lo lo is at most 2^-22 of the product, of
 // either sign.  The floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39.
-// b is kept without c0 I, and while four or more steps follow x is carried in fp32 beside its
+// b is kept without c0 I, and in the first step and while four or more follow x is carried in fp32 beside its
 // pairs: early steps are little more than x = c0 x, and what is lost of a small singular value there
 // is enlarged by every later step (final error on a 1024 x 1024 gradient: 4.2e-7 carried to the end,
 // 5.2e-7 so, 7.8e-7 never; fp32 products give 1.3e-6).
@@ -871,8 +871,9 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
         k.q = xt[s & 1];
         k.carried = carried;
         k.was_t = xt[s & 1];
-        // what an error in x grows to depends on the steps that follow: x in 32 bits while four or more do
-        k.from_carried = steps - s >= 4;
+        // what an error in x grows to depends on the steps that follow: x in 32 bits while four or more do, and in the
+        // first step, whose x lies there in 32 bits whatever follows
+        k.from_carried = s == 0 || steps - s >= 4;
         k.to_carried = steps - s >= 5;
         k.a_unscale = 1.f / up_x;
         k.out = x;

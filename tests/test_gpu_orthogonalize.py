@@ -296,3 +296,18 @@ def test_orthogonalize_at_the_ends_of_one_launch(shape):
     out = tl.orthogonalize(three.cuda())
     for i in range(3):
         _check(out[i], three[i], 5)
+
+
+@pytest.mark.parametrize("shape", [(300, 500), (700, 260), (3, 200, 330), (1, 5000), (40, 60)], ids=lambda s: "x".join(map(str, s)))
+def test_the_first_step_reads_x_in_32_bits(shape):
+    """With b = 0 a step is x = c0 x: x0's rounding and the product's, whatever the size of a row beside the others'."""
+    for tall in (False, True):
+        g = torch.randn(shape, generator=torch.Generator().manual_seed(4))
+        if shape[-2] > 1:
+            g[..., ::3, :] *= 1e-6
+        g = g.transpose(-2, -1).contiguous() if tall else g
+        print(f"orthogonalize c0 alone {tuple(g.shape)}", flush=True)
+        out = tl.orthogonalize(g.cuda(), steps=1, coefficients=(1.5, 0.0, 0.0)).double().cpu()
+        want = g.double()
+        want = 1.5 * want / (want.square().sum((-2, -1), keepdim=True).sqrt() + 1e-7)
+        assert bool(((out - want).abs() <= 2.0 ** -23 * (1 + 2.0 ** -20) * want.abs()).all())
