@@ -269,6 +269,7 @@ __global__ __launch_bounds__(NT * MT == 1 ? 1024 : 512) void linear_q4_stream_ke
         for (int w = 0; w < waves; ++w)
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) v += red[(w * rows + m * PIECES + p) * WIDTH + c];
+        v *= 1 / Codes<TYPE>::UNIT;
         if (a.bias) v += (float)static_cast<const T*>(a.bias)[n];
         static_cast<T*>(a.y)[(size_t)m * a.lay.N + n] = (T)v;
     }

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void linear_q4_records_kernel(BandArgs a)
         for (int p = 0; p < R::PIECES; ++p)
             *reinterpret_cast<uintx4*>(to + ((tile * R::STEPS + i) * R::PIECES + p) * 1024 + lane * 16) = piece_of<TYPE>(v, p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += (float)v[e];
+        for (int e = 0; e < 8; ++e) sum += (float)v[e] * Codes<TYPE>::UNIT;
         if ((i + 1) % (R::STEPS / GROUPS) == 0) {   // the end of a run
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
@@ -311,12 +311,12 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
             if (a.partial) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (m + r < a.M) a.partial[((size_t)slice * a.M + m + r) * a.lay.N + n] = acc[mt][nt][r];
+                    if (m + r < a.M) a.partial[((size_t)slice * a.M + m + r) * a.lay.N + n] = acc[mt][nt][r] * (1 / Codes<TYPE>::UNIT);
             } else {
                 const float bias = a.bias ? (float)static_cast<const T*>(a.bias)[n] : 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (m + r < a.M) static_cast<T*>(a.y)[(size_t)(m + r) * a.lay.N + n] = (T)(acc[mt][nt][r] + bias);
+                    if (m + r < a.M) static_cast<T*>(a.y)[(size_t)(m + r) * a.lay.N + n] = (T)(acc[mt][nt][r] * (1 / Codes<TYPE>::UNIT) + bias);
             }
         }
     }

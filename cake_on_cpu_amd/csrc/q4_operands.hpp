@@ -4,7 +4,10 @@
 // Codes are whole numbers 0..15, exact in 16-bit floats, so the products go to the matrix pipe as
 // x . code and the group's scale and zero point are applied to the 32-bit sums behind it:
 //   y[m][n] = sum over groups g of s[n][g] * (sum_k x[m][k] code[n][k] - z[n][g] * sum_k x[m][k]).
-// No weight is rounded.  x is exact as well: 16-bit types go in as they are, a 32-bit x as three
+// No weight is rounded.  The sums are larger than what they stand for, up to 15 x 128 of the largest x before the
+// scale is applied, so where x reaches as far as fp32 does, codes and column sums count in units of 2^-12
+// (exact, by the unpacking's own scale) and the result is multiplied by 2^12 at its end: no sum overflows where the
+// values do not.  x is exact as well: 16-bit types go in as they are, a 32-bit x as three
 // bf16 pieces (its leading, middle and last 8 significant bits, cut, not rounded, so that no piece
 // overflows) that take three rows of the product and are added up at the end.
 #pragma once
@@ -13,15 +16,16 @@
 
 namespace cake {
 
-template <int TYPE> struct Codes;   // what the matrix pipe multiplies
+template <int TYPE> struct Codes;   // what the matrix pipe multiplies: code * UNIT
 template <> struct Codes<CAKE_HIP_F16> {
     typedef f16x8 V;
+    static constexpr float UNIT = 1.f, UNPACK = 512.f * UNIT;
     static __device__ __forceinline__ unsigned pair(unsigned bytes, bool upper)
     {
-        return upper ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.f, true))
-                     : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.f, false));
+        return upper ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, UNPACK, true))
+                     : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, UNPACK, false));
     }
-    static constexpr unsigned ONES = 0x3C003C00u;
+    static constexpr unsigned ONES = 0x3C003C00u;   // UNIT
     static __device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
@@ -29,12 +33,13 @@ template <> struct Codes<CAKE_HIP_F16> {
 };
 template <> struct Codes<CAKE_HIP_BF16> {
     typedef bf16x8 V;
+    static constexpr float UNIT = 0x1p-12f, UNPACK = 512.f * UNIT;
     static __device__ __forceinline__ unsigned pair(unsigned bytes, bool upper)
     {
-        return upper ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.f, true))
-                     : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.f, false));
+        return upper ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, UNPACK, true))
+                     : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, UNPACK, false));
     }
-    static constexpr unsigned ONES = 0x3F803F80u;
+    static constexpr unsigned ONES = 0x39803980u;   // UNIT
     static __device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);

@@ -405,3 +405,18 @@ def test_few_rows_of_every_number_and_many_outputs(kind):
             print(f"linear_q4 M={M} K={K} {kind}", flush=True)
             x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(TYPES[kind]).cuda()
             _check(tl.forward_q4(x, q), x, v64, mass, None, K)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_an_input_of_huge_values(kind):
+    """Products of x and whole codes, or the sum of a row of x, pass 32 bits long before what they stand for does."""
+    N, K = 40, 300
+    for group, zeros in ((32, True), (64, False), (128, True), (128, False)):
+        packed, s, z, v64, mass = _weights(N, K, group, zeros, torch.float32, 5)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+        for M in (1, 4, 9, 20, 30, 70, 200):
+            x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).clamp(-3, 3)
+            x = (x * (2.5e38 / float((x.double().abs() @ v64.abs().t()).max()))).to(TYPES[kind])      # no order of the sums overflows
+            assert float(x.abs().max()) > 1e36
+            print(f"linear_q4 huge M={M} {kind} group={group} zeros={zeros}", flush=True)
+            _check(tl.forward_q4(x.cuda(), q), x, v64, mass, None, K)
