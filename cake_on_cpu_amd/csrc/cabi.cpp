@@ -2375,7 +2375,7 @@ static int orthogonalize_dims_ok(int batch, int rows, int cols)
 size_t cake_hip_orthogonalize_workspace(int batch, int rows, int cols)
 {
     if (orthogonalize_dims_ok(batch, rows, cols) || batch == 0 || rows == 0 || cols == 0) return 0;
-    return orthogonalize_layout(batch, rows, cols).bytes;
+    return orthogonalize_workspace(batch, rows, cols);
 }
 
 int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1,
@@ -2401,7 +2401,7 @@ int cake_hip_orthogonalize(const void* g, void* out, int type, int batch, int ro
     if ((st = any_in(g, bytes, 0, true, &in, "g"))) return st;
     if ((st = any_in(out, bytes, 1, false, &res, "out"))) return st;
     void* ws = nullptr;
-    if ((st = workspace_of(workspace, orthogonalize_layout(batch, rows, cols).bytes, 256, cur().orthogonal, &ws))) return st;
+    if ((st = workspace_of(workspace, orthogonalize_workspace(batch, rows, cols), 256, cur().orthogonal, &ws))) return st;
     Timer timer(stream, seconds);
     if ((st = timer.start())) return st;
     st = timer.family(0, [&] {

@@ -291,18 +291,12 @@ size_t linear_q4_bands_workspace(int M, int N, int K, int type);
 hipError_t launch_linear_q4_bands(const void* x, const void* q, const void* bias, void* y, int type, int M, const Q4Layout& lay,
                                   bool with_zeros, void* workspace, hipStream_t stream);
 
-// Newton-Schulz iterations (orthogonalize.hip).  The layout's offsets are bytes into the workspace.
-struct OrthogonalizeLayout {
-    int m, n;                     // the shorter and the longer side
-    int mb, nb;                   // in blocks of 16, even
-    size_t x_halves, a_halves;    // of one matrix of the batch; the carried x has x_halves / 2 floats
-    size_t x, xt0, xt1, a, b, partial, carried, slices, bytes;
-};
+// Newton-Schulz iterations (orthogonalize.hip)
 // powers of two that the values of x, a and b are multiplied by where they are kept
 struct OrthogonalizeScales {
     int ex, ea, eb;
 };
-OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols);
+size_t orthogonalize_workspace(int batch, int rows, int cols);   // bytes, of a batch of one or more
 hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1,
                                 double c2, double eps, const OrthogonalizeScales& sc, void* workspace, hipStream_t stream);
 

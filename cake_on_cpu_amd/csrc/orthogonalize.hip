@@ -781,7 +781,16 @@ bool small_fits(int mb, int nb)
 
 }  // namespace
 
-OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols)
+namespace {
+
+struct OrthogonalizeLayout {      // of one pass; offsets are bytes into the workspace
+    int m, n;                     // the shorter and the longer side
+    int mb, nb;                   // in blocks of 16, even
+    size_t x_halves, a_halves;    // of one matrix of the batch; the carried x has x_halves / 2 floats
+    size_t x, xt0, xt1, a, b, partial, carried, slices, bytes;
+};
+
+OrthogonalizeLayout layout_of(int batch, int rows, int cols)
 {
     OrthogonalizeLayout l;
     l.m = rows < cols ? rows : cols;
@@ -804,10 +813,52 @@ OrthogonalizeLayout orthogonalize_layout(int batch, int rows, int cols)
     return l;
 }
 
+// Matrices beyond PASS_VALUES together are taken some at a time, as evenly as they divide: the workspace holds 16 to
+// 24 bytes a value, and a device that is full gains nothing from more (8 of 4096 x 4096 take 28.2 ms, 8 times one of them; 16
+// of 1024 x 4096, which one pass takes, 4.2 ms, 16 of them by themselves 6.5).
+constexpr size_t PASS_VALUES = (size_t)1 << 26;
+
+int passes_of(int batch, int rows, int cols)
+{
+    const OrthogonalizeLayout one = layout_of(1, rows, cols);
+    if (small_fits(one.mb, one.nb)) return 1;
+    const size_t values = (size_t)one.mb * one.nb * 256;
+    const size_t most = values < PASS_VALUES ? PASS_VALUES / values : 1;
+    return (int)((batch + most - 1) / most);
+}
+
+hipError_t launch_pass(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1, double c2, double eps,
+                       const OrthogonalizeScales& sc, void* workspace, hipStream_t stream);
+
+}  // namespace
+
+size_t orthogonalize_workspace(int batch, int rows, int cols)
+{
+    const int passes = passes_of(batch, rows, cols);
+    // a pass of one matrix less may ask for more slices
+    return std::max(layout_of(batch / passes, rows, cols).bytes, layout_of((batch + passes - 1) / passes, rows, cols).bytes);
+}
+
 hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1,
                                 double c2, double eps, const OrthogonalizeScales& sc, void* workspace, hipStream_t stream)
 {
-    const OrthogonalizeLayout l = orthogonalize_layout(batch, rows, cols);
+    const int passes = passes_of(batch, rows, cols);
+    const size_t bytes = (size_t)rows * cols * type_bytes(type);
+    for (int p = 0; p < passes; ++p) {
+        const int from = (int)((long long)batch * p / passes), to = (int)((long long)batch * (p + 1) / passes);
+        const hipError_t e = launch_pass(static_cast<const char*>(g) + from * bytes, static_cast<char*>(out) + from * bytes, type, to - from, rows, cols,
+                                         steps, c0, c1, c2, eps, sc, workspace, stream);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+namespace {
+
+hipError_t launch_pass(const void* g, void* out, int type, int batch, int rows, int cols, int steps, double c0, double c1, double c2, double eps,
+                       const OrthogonalizeScales& sc, void* workspace, hipStream_t stream)
+{
+    const OrthogonalizeLayout l = layout_of(batch, rows, cols);
     const float up_x = ldexpf(1.f, sc.ex), up_a = ldexpf(1.f, sc.ea), up_b = ldexpf(1.f, sc.eb);
     const bool tall = rows > cols;
     if (small_fits(l.mb, l.nb)) {
@@ -892,5 +943,7 @@ hipError_t launch_orthogonalize(const void* g, void* out, int type, int batch, i
     }
     return hipSuccess;
 }
+
+}  // namespace
 
 }  // namespace cake

@@ -471,6 +471,8 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
  * 2^-23 of each value and no finer than 2^-39 (for the coefficients above), so a g whose
  * norm lies below about 1e-4 eps loses relative accuracy.  A matrix of zeros gives zeros; one that holds a NaN
  * or an infinity gives NaN and leaves the rest of the batch alone.
+ * Matrices of more than 2^26 values together are taken some at a time, so the workspace stays within some 1.5 GB or what one
+ * matrix needs (16 to 24 bytes a value).
  * workspace: device memory of cake_hip_orthogonalize_workspace bytes (0 for small matrices), 256-byte
  * aligned, or NULL for a buffer of the context's own; calls that overlap need workspaces of their own. */
 size_t cake_hip_orthogonalize_workspace(int batch, int rows, int cols);

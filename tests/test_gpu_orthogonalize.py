@@ -311,3 +311,33 @@ def test_the_first_step_reads_x_in_32_bits(shape):
         want = g.double()
         want = 1.5 * want / (want.square().sum((-2, -1), keepdim=True).sqrt() + 1e-7)
         assert bool(((out - want).abs() <= 2.0 ** -23 * (1 + 2.0 ** -20) * want.abs()).all())
+
+
+@pytest.mark.parametrize("shape", [(37, 1024, 2048), (35, 2048, 1000), (3, 6000, 5700)], ids=lambda s: "x".join(map(str, s)))
+def test_a_batch_taken_in_passes(shape):
+    """More values than one pass takes (37 matrices in 19 and 18, three singly): every matrix against the 64-bit iteration,
+    in place as well, and nothing behind the last one is written."""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB of device memory")
+    batch, m, n = shape
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    room = torch.full((batch * m * n + 64,), 7.0, device="cuda")
+    out = room[:-64].view(shape)
+    g = torch.randn(shape, device="cuda", generator=gen) * torch.logspace(-4, 4, batch, device="cuda")[:, None, None]
+    print(f"orthogonalize in passes {shape}", flush=True)
+    ws = torch.empty(cake.orthogonalize_workspace(*shape), dtype=torch.uint8, device="cuda")
+    cake.orthogonalize(g, out, *shape, steps=2, workspace=ws, timed=False)
+    assert torch.equal(tl.orthogonalize(g, steps=2), out) and bool((room[-64:] == 7).all())
+    for i in range(batch):
+        x = g[i].double() if m <= n else g[i].double().t().contiguous()
+        x = x / (x.norm() + 1e-7)
+        bar = float(x.norm()) * 3.4445 ** 2
+        for step in (1, 2):
+            a = x @ x.t().contiguous()
+            x = USUAL[0] * x + (USUAL[1] * a + USUAL[2] * (a @ a)) @ x
+            bar += float(x.norm()) * 3.4445 ** (2 - step)
+        assert float((out[i].double() - (x if m <= n else x.t())).norm()) <= 32 * 2.0 ** -24 * bar, i
+    cake.orthogonalize(g, g, *shape, steps=2, workspace=ws, timed=False)
+    assert torch.equal(g, out)
+    del room, out, g, ws, x, a
+    torch.cuda.empty_cache()

@@ -238,3 +238,12 @@ def test_a_refused_load_changes_nothing():
     assert bool((model[0].packed == 2).all())
     with pytest.raises(RuntimeError):       # strict: what the bytes were made for has to be there
         model.load_state_dict({k: v for k, v in other.state_dict().items() if "extra" not in k})
+
+
+def test_a_workspace_does_not_grow_with_the_number_of_large_matrices():
+    """Beyond 2^26 values a batch is taken some matrices at a time: 16 bytes a value of a pass (x three times in
+    pairs, once in fp32), 8 a value of its squares, and the sums of slices."""
+    ws = cake.orthogonalize_workspace
+    assert ws(64, 4096, 4096) <= 1.1 * 24 * 2 ** 26 and ws(4, 4096, 4096) >= 20 * 2 ** 26
+    assert ws(32, 14336, 4096) == ws(1, 14336, 4096) and ws(65535, 300, 300) <= 1.1 * 24 * 2 ** 26
+    assert ws(65535, 64, 64) == 0
