@@ -308,7 +308,9 @@ class cake_muon(torch.optim.Optimizer):
     other vectors belong to another optimiser):
         b = momentum * b + grad,  u = grad + momentum * b  (b without nesterov)
         w = w - lr * weight_decay * w - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
-    Matrices of one shape are orthogonalised in one call."""
+    Matrices of one shape are orthogonalised together.  The state is kept in fp32 whatever the parameters' type (float32,
+    float16, bfloat16): the momentum, and of a 16-bit w an fp32 copy that the formula runs on and w is rounded from, so that
+    updates below a step of w's type add up.  A w that was set from elsewhere counts as it was set."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=api.NEWTON_SCHULZ,
                  eps=1e-7):
@@ -325,6 +327,21 @@ class cake_muon(torch.optim.Optimizer):
                     raise ValueError(f"cake_muon: parameter {tuple(w.shape)} is no matrix")
         super().add_param_group({**param_group, "params": params})
 
+    def load_state_dict(self, state_dict):
+        """As the base class does, but without rounding the state to the parameters' type."""
+        given = []
+        hook = self.register_load_state_dict_pre_hook(lambda _, d: given.append(d))   # what other hooks made of it
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        given = given[-1]
+        names = [n for group in given["param_groups"] for n in group["params"]]
+        for n, w in zip(names, (w for group in self.param_groups for w in group["params"])):
+            for key, value in given["state"].get(n, {}).items():
+                if isinstance(value, torch.Tensor):
+                    self.state[w][key] = value.detach().to(device=w.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -334,20 +351,37 @@ class cake_muon(torch.optim.Optimizer):
         for group in self.param_groups:
             alike = {}
             for w in group["params"]:
-                if w.grad is None or w.numel() == 0:
-                    continue
-                state = self.state[w]
-                if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(w)
-                b = state["momentum"].mul_(group["momentum"]).add_(w.grad)
-                u = w.grad.add(b, alpha=group["momentum"]) if group["nesterov"] else b
-                alike.setdefault((tuple(w.shape), w.dtype, w.device), []).append((w, u))
-            for (shape, _, _), pairs in alike.items():
-                us = torch.stack([u for _, u in pairs]) if len(pairs) > 1 else pairs[0][1].unsqueeze(0)
-                done = orthogonalize(us, group["steps"], group["coefficients"], group["eps"])
-                scale = max(1.0, shape[0] / shape[1]) ** 0.5
-                for i, (w, _) in enumerate(pairs):
-                    if group["weight_decay"]:
-                        w.mul_(1 - group["lr"] * group["weight_decay"])
-                    w.add_(done[i], alpha=-group["lr"] * scale)
+                if w.grad is not None and w.numel() != 0:
+                    alike.setdefault((tuple(w.shape), w.dtype, w.device), []).append(w)
+            for ws in alike.values():
+                self._update(group, ws)
         return loss
+
+    def _update(self, group, ws):
+        rows, cols = ws[0].shape
+        momentum, rate = group["momentum"], group["lr"] * max(1.0, rows / cols) ** 0.5
+        us = torch.empty((len(ws), rows, cols), dtype=torch.float32, device=ws[0].device)
+        for u, w in zip(us, ws):
+            state = self.state[w]
+            if "momentum" not in state:
+                state["momentum"] = torch.zeros_like(w, dtype=torch.float32)
+            b = state["momentum"].mul_(momentum).add_(w.grad)
+            if group["nesterov"]:
+                torch.add(w.grad, b, alpha=momentum, out=u)
+            else:
+                u.copy_(b)
+        for w, done in zip(ws, orthogonalize(us, group["steps"], group["coefficients"], group["eps"])):
+            full = w if w.dtype == torch.float32 else self._in_32_bits(w)
+            if group["weight_decay"]:
+                full.mul_(1 - group["lr"] * group["weight_decay"])
+            full.add_(done, alpha=-rate)
+            if full is not w:
+                w.copy_(full)
+
+    def _in_32_bits(self, w):
+        state = self.state[w]
+        if "weight" not in state:
+            state["weight"] = w.float()
+        else:   # entries that are no longer what was rounded from here
+            state["weight"].copy_(torch.where(state["weight"].to(w.dtype) == w, state["weight"], w.float()))
+        return state["weight"]

@@ -130,3 +130,114 @@ def test_a_call_names_torchs_default_stream(monkeypatch):
         for Torch._C.handle, want in ((0, _lib.NULL_STREAM), (0x1234, 0x1234)):
             assert api._torch_stream(Torch, device) == want
     assert _lib.NULL_STREAM != 0 and api._stream(np.zeros(1, np.float32), torch.zeros(1)) == 0   # host operands: the context's own
+
+
+@pytest.fixture
+def signs(monkeypatch):
+    """In place of the iterations something as blunt that torch computes the same everywhere; returns the calls' batches."""
+    calls = []
+
+    def orthogonalize(g, out, batch, rows, cols, steps, coefficients, eps, workspace=None, timed=True):
+        assert g.shape == out.shape and g.dtype == out.dtype and g.is_contiguous()
+        calls.append((batch, rows, cols, g.dtype))
+        out.copy_(g.sign() * 0.25)
+
+    monkeypatch.setattr(api, "orthogonalize", orthogonalize)
+    return calls
+
+
+def _grads(shape, dtype, steps, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(shape, generator=gen).to(dtype) for _ in range(steps)]
+
+
+def _formula(w, grads, lr, mu, nesterov, decay):
+    """The optimiser's formula in 64 bits on the stand-in: weights and momentum after every step"""
+    w, b, out = w.double(), torch.zeros_like(w, dtype=torch.float64), []
+    for g in grads:
+        b = mu * b + g.double()
+        u = g.double() + mu * b if nesterov else b
+        w = w - lr * decay * w - lr * max(1.0, w.size(0) / w.size(1)) ** 0.5 * u.sign() * 0.25
+        out.append((w, b))
+    return out
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_optimiser_keeps_its_state_in_32_bits(signs, dtype, nesterov):
+    """200 steps of every type of parameter against the formula: momentum to 32 bits (two roundings a step of at most the
+    largest |b|, of which 1 / (1 - mu) count together), a 16-bit weight to one rounding of the formula's."""
+    start, lr, mu, decay = torch.randn(7, 3, generator=torch.Generator().manual_seed(3)).to(dtype), 0.01, 0.95, 0.1
+    w = torch.nn.Parameter(start.clone())
+    opt = tl.cake_muon([w], lr=lr, momentum=mu, nesterov=nesterov, weight_decay=decay)
+    grads = _grads((7, 3), dtype, 200)
+    formula = _formula(start, grads, lr, mu, nesterov, decay)
+    widest = max(float(b.abs().max()) for _, b in formula)
+    for i, (g, (want, b)) in enumerate(zip(grads, formula)):
+        w.grad = g.clone()
+        opt.step()
+        held = opt.state[w]["momentum"]
+        assert held.dtype == torch.float32
+        assert float((held.double() - b).abs().max()) <= 2 * 2.0 ** -24 * widest / (1 - mu), i
+        # two roundings of a step of the 32-bit weight, 200 steps of values below 4, then the type's
+        bar = 2 * (i + 1) * 2.0 ** -24 * 4 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * (want.abs() + 1e-4))
+        assert bool(((w.detach().double() - want).abs() <= bar).all()), i
+    assert all(c[3] == torch.float32 for c in signs)
+
+
+def test_decay_below_a_16_bit_step_is_not_lost(signs):
+    """1000 steps of weights w = w - 0.001 w: every single one is below half a step of bfloat16."""
+    w = torch.nn.Parameter(torch.ones(4, 4, dtype=torch.bfloat16))
+    opt = tl.cake_muon([w], lr=0.01, weight_decay=0.1)
+    for _ in range(1000):
+        w.grad = torch.zeros_like(w)
+        opt.step()
+    assert bool(((w.detach().double() - 0.999 ** 1000).abs() <= 2.0 ** -9 * 0.37).all())
+
+
+def test_a_16_bit_weight_set_from_elsewhere_is_what_counts(signs):
+    """Loaded or clipped weights are not undone by what the optimiser kept of the old ones."""
+    w = torch.nn.Parameter(torch.ones(4, 4, dtype=torch.bfloat16))
+    opt = tl.cake_muon([w], lr=0.0, momentum=0.0, weight_decay=0.0)
+    for _ in range(3):
+        w.grad = torch.ones_like(w)
+        opt.step()
+    with torch.no_grad():
+        w[1].fill_(-2.0)
+        w[2, 2] = float("nan")
+    opt.step()
+    want = torch.ones(4, 4)
+    want[1] = -2.0
+    want[2, 2] = float("nan")
+    assert torch.equal(w.detach().float().nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_stored_optimiser_goes_on_where_it_was(signs, tmp_path, dtype):
+    """Loading does not round the state to the parameters' type, whatever group a parameter is in."""
+    def made():
+        ws = [torch.nn.Parameter(torch.full(s, 0.5, dtype=dtype)) for s in ((4, 6), (6, 4), (4, 6))]
+        return ws, tl.cake_muon([{"params": ws[:1]}, {"params": ws[1:], "lr": 0.003}], lr=0.01, weight_decay=0.05)
+
+    def steps(ws, opt, seeds):
+        for seed in seeds:
+            for i, w in enumerate(ws):
+                w.grad = _grads(tuple(w.shape), dtype, 1, 10 * seed + i)[0]
+            opt.step()
+
+    ws, opt = made()
+    steps(ws, opt, range(5))
+    torch.save((opt.state_dict(), [w.detach() for w in ws]), tmp_path / "o")
+    held, weights = torch.load(tmp_path / "o", weights_only=True)
+    others, other = made()
+    with torch.no_grad():
+        for a, b in zip(others, weights):
+            a.copy_(b)
+    other.load_state_dict(held)
+    for a, b in zip(ws, others):
+        assert all(torch.equal(opt.state[a][k], other.state[b][k]) and other.state[b][k].dtype == torch.float32 for k in opt.state[a])
+    steps(ws, opt, range(5, 9))
+    steps(others, other, range(5, 9))
+    assert all(torch.equal(a, b) for a, b in zip(ws, others))
+    kept = held["state"][0]["momentum"].clone()
+    assert torch.equal(kept, torch.load(tmp_path / "o", weights_only=True)[0]["state"][0]["momentum"])   # and steps do not reach into what was loaded
