@@ -303,12 +303,16 @@ def _orthogonalize(grad, steps, coefficients, eps):
     return out
 
 
+# Values of matrices that the optimiser copies together for one call: what the library takes in one pass, too
+_TOGETHER = 1 << 26
+
+
 class cake_muon(torch.optim.Optimizer):
     """Momentum with orthogonalised updates for weight matrices (cake_linear.weight and the like; biases and
     other vectors belong to another optimiser):
         b = momentum * b + grad,  u = grad + momentum * b  (b without nesterov)
         w = w - lr * weight_decay * w - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
-    Matrices of one shape are orthogonalised together.  The state is kept in fp32 whatever the parameters' type (float32,
+    Matrices of one shape are orthogonalised together, up to 2^26 values in a call.  The state is kept in fp32 whatever the parameters' type (float32,
     float16, bfloat16): the momentum, and of a 16-bit w an fp32 copy that the formula runs on and w is rounded from, so that
     updates below a step of w's type add up.  A w that was set from elsewhere counts as it was set."""
 
@@ -353,8 +357,10 @@ class cake_muon(torch.optim.Optimizer):
             for w in group["params"]:
                 if w.grad is not None and w.numel() != 0:
                     alike.setdefault((tuple(w.shape), w.dtype, w.device), []).append(w)
-            for ws in alike.values():
-                self._update(group, ws)
+            for (shape, _, _), ws in alike.items():
+                some = max(1, _TOGETHER // (shape[0] * shape[1]))
+                for i in range(0, len(ws), some):
+                    self._update(group, ws[i:i + some])
         return loss
 
     def _update(self, group, ws):

@@ -241,3 +241,14 @@ def test_a_stored_optimiser_goes_on_where_it_was(signs, tmp_path, dtype):
     assert all(torch.equal(a, b) for a, b in zip(ws, others))
     kept = held["state"][0]["momentum"].clone()
     assert torch.equal(kept, torch.load(tmp_path / "o", weights_only=True)[0]["state"][0]["momentum"])   # and steps do not reach into what was loaded
+
+
+def test_the_optimisers_copies_do_not_grow_with_the_number_of_large_matrices(signs):
+    """Matrices of one shape go together up to 2^26 values."""
+    ws = [torch.nn.Parameter(torch.zeros(2048, 4096)) for _ in range(11)] + [torch.nn.Parameter(torch.zeros(3, 5)) for _ in range(7)]
+    opt = tl.cake_muon(ws, lr=1.0, momentum=0.0)
+    for i, w in enumerate(ws):
+        w.grad = torch.full_like(w, 1.0 if i % 3 else -1.0)
+    opt.step()
+    assert [c[0] for c in signs] == [8, 3, 7]
+    assert all(bool((w == (-0.25 if i % 3 else 0.25)).all()) for i, w in enumerate(ws))
