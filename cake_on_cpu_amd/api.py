@@ -662,6 +662,12 @@ def orthogonalize_workspace(batch, rows, cols) -> int:
     return load().cake_hip_orthogonalize_workspace(batch, rows, cols)
 
 
+def orthogonalize_check(steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7) -> None:
+    """Raises for what orthogonalize refuses whatever the matrices."""
+    c0, c1, c2 = coefficients
+    check(load().cake_hip_orthogonalize(None, None, _lib.F32, 0, 0, 0, steps, c0, c1, c2, eps, None, None, None), "orthogonalize")
+
+
 def orthogonalize(g, out, batch, rows, cols, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, workspace=None, timed=True) -> float:
     """Newton-Schulz iterations on g[batch][rows][cols] into out (of g's element type; may be g):
     x = g / (|g| + eps), then `steps` times a = x x^T, x = c0 x + (c1 a + c2 a a) x.

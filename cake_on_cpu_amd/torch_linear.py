@@ -352,6 +352,7 @@ class cake_muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check()
         for group in self.param_groups:
             alike = {}
             for w in group["params"]:
@@ -362,6 +363,19 @@ class cake_muon(torch.optim.Optimizer):
                 for i in range(0, len(ws), some):
                     self._update(group, ws[i:i + some])
         return loss
+
+    def _check(self):
+        """Raises for what cannot be taken, before anything is changed."""
+        for group in self.param_groups:
+            api.orthogonalize_check(group["steps"], group["coefficients"], group["eps"])
+            for w in group["params"]:
+                if w.grad is None or w.numel() == 0:
+                    continue
+                if w.grad.layout != torch.strided or w.grad.shape != w.shape:
+                    raise TypeError(f"cake_muon: gradient {tuple(w.grad.shape)} of {w.grad.layout} for a matrix {tuple(w.shape)}")
+                api.element_type(w.dtype)
+                if w.is_cuda and w.device.index != api.device_info().device:
+                    raise ValueError(f"cake_muon: parameter on {w.device}, the library works on device {api.device_info().device}")
 
     def _update(self, group, ws):
         rows, cols = ws[0].shape

@@ -252,3 +252,26 @@ def test_the_optimisers_copies_do_not_grow_with_the_number_of_large_matrices(sig
     opt.step()
     assert [c[0] for c in signs] == [8, 3, 7]
     assert all(bool((w == (-0.25 if i % 3 else 0.25)).all()) for i, w in enumerate(ws))
+
+
+def test_a_refused_step_changes_nothing(signs):
+    a, b = torch.nn.Parameter(torch.ones(3, 4)), torch.nn.Parameter(torch.ones(4, 4))
+    for bad, error in ((dict(steps=0), cake.CakeHipError), (dict(steps=1001), cake.CakeHipError), (dict(coefficients=(40.0, 0.0, 0.0)), cake.CakeHipError),
+                       (dict(eps=-1.0), cake.CakeHipError), (dict(coefficients=(1.0, 2.0)), ValueError)):
+        opt = tl.cake_muon([{"params": [a]}, {"params": [b], **bad}])
+        a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+        with pytest.raises(error):
+            opt.step()
+        assert bool((a == 1).all()) and not opt.state
+    for other in (torch.nn.Parameter(torch.ones(4, 4, dtype=torch.float64)), torch.nn.Parameter(torch.ones(4, 4, dtype=torch.complex64))):
+        opt = tl.cake_muon([a, other])
+        other.grad = torch.ones_like(other)
+        with pytest.raises(TypeError):
+            opt.step()
+        assert bool((a == 1).all()) and not opt.state
+    opt = tl.cake_muon([a, b])
+    b.grad = torch.ones(4, 4).to_sparse()
+    with pytest.raises(TypeError):
+        opt.step()
+    assert bool((a == 1).all()) and not opt.state
+    assert not signs
