@@ -551,14 +551,22 @@ def _any_ptr(a, what: str, of: int | None = None) -> int:
 class Q4Weight:
     """A weight matrix v[N][K] in 4 bits, v = (code - zero) * scale per run of `group` columns: the packed
     bytes (numpy or torch uint8, in the library's own order) and what they hold.  It is made by q4_pack
-    or q4_quantize; q4_of wraps bytes that were stored."""
-    __slots__ = ("data", "N", "K", "group", "scale_type", "with_zeros")
+    or q4_quantize; q4_of wraps bytes that were stored.  What it holds does not change: other bytes are
+    another Q4Weight."""
+    __slots__ = ("data", "N", "K", "group", "scale_type", "with_zeros", "bytes")
 
     def __init__(self, data, N, K, group, scale_type, with_zeros):
         _any_ptr(data, "packed weights")
-        _need(data, _q4_bytes(N, K, group, scale_type, with_zeros), "packed weights")
-        self.data, self.N, self.K, self.group = data, N, K, group
-        self.scale_type, self.with_zeros = scale_type, bool(with_zeros)
+        size = _q4_bytes(N, K, group, scale_type, with_zeros)
+        _need(data, size, "packed weights")
+        for name, value in zip(self.__slots__, (data, N, K, group, scale_type, bool(with_zeros), size)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"packed weights are made for one {name}; q4_of wraps other bytes")
+
+    def __reduce__(self):
+        return Q4Weight, (self.data, self.N, self.K, self.group, self.scale_type, self.with_zeros)
 
 
 def _q4_bytes(N, K, group, scale_type, zeros) -> int:
@@ -620,6 +628,7 @@ def q4_quantize(w, N, K, group=128, zeros=False, scale_dtype="float32", timed=Fa
 def q4_dequantize(q: Q4Weight, w, timed=False) -> float:
     """The values that packed weights stand for, into w[N][K] of any element type.  Returns seconds (0 with timed=False)."""
     _need(w, q.N * q.K, "w")
+    _need(q.data, q.bytes, "packed weights")
     wt = element_type(w.dtype)
     secs = C.c_double(0.0)
     check(load().cake_hip_q4_dequantize(_any_ptr(q.data, "q"), _any_ptr(w, "w", wt), wt, q.N, q.K, q.group, q.scale_type,
@@ -641,6 +650,7 @@ def linear_q4_forward(x, q: Q4Weight, bias, y, M, workspace=None, timed=True) ->
     N, K = q.N, q.K
     _need(x, M * K, "x")
     _need(y, M * N, "y")
+    _need(q.data, q.bytes, "packed weights")
     if bias is not None:
         _need(bias, N, "bias")
     if workspace is not None:

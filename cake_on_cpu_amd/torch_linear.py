@@ -176,6 +176,8 @@ def _forward_q4(input, q, bias):
         raise ValueError(f"forward_q4: input {tuple(input.shape)} does not match {q.K} columns of weights")
     if not q.data.is_contiguous():
         raise TypeError("forward_q4: packed weights must be contiguous")
+    if q.data.numel() < q.bytes:   # resized since they were made
+        raise ValueError(f"forward_q4: packed weights hold {q.data.numel()} bytes, {q.bytes} needed")
     if bias is not None and (tuple(bias.shape) != (q.N,) or bias.dtype != input.dtype):
         raise ValueError(f"forward_q4: bias {tuple(bias.shape)} of {bias.dtype} does not match {q.N} outputs of {input.dtype}")
     if input.device != q.data.device or (bias is not None and bias.device != input.device):

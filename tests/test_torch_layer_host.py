@@ -275,3 +275,36 @@ def test_a_refused_step_changes_nothing(signs):
         opt.step()
     assert bool((a == 1).all()) and not opt.state
     assert not signs
+
+
+def test_packed_weights_stay_what_they_were_made_as(stand_in):
+    """What a kernel reads follows from these numbers, so they do not change behind their check; bytes that shrank are refused."""
+    q = cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    for name, value in (("data", torch.zeros(16, dtype=torch.uint8)), ("N", 500), ("K", 64), ("group", 64), ("scale_type", 1), ("with_zeros", True)):
+        with pytest.raises(AttributeError):
+            setattr(q, name, value)
+    x = torch.ones(2, K)
+    tl.forward_q4(x, q)
+    q.data.resize_(q.data.numel() - 1)
+    for call in (lambda: tl.forward_q4(x, q), lambda: tl.forward_q4(x.clone().requires_grad_(), q), lambda: tl.dequantize_q4(q)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_shrunk_bytes_are_refused_by_the_plain_interface():
+    q = cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    q.data.resize_(q.data.numel() - 1)
+    x, y = torch.ones(2, K), torch.full((2, N), 7.0)
+    for call in (lambda: cake.linear_q4_forward(x, q, None, y, 2), lambda: cake.q4_dequantize(q, torch.zeros(N, K))):
+        with pytest.raises(ValueError):
+            call()
+    assert bool((y == 7).all())
+
+
+def test_packed_weights_are_copied_and_stored_whole():
+    import copy
+    import pickle
+    q = cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert torch.equal(other.data, q.data) and (other.N, other.K, other.group, other.scale_type, other.with_zeros) == (N, K, 32, _lib.F32, False)
+    assert copy.deepcopy(q).data.data_ptr() != q.data.data_ptr()
