@@ -117,10 +117,10 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
     typedef typename Element<TYPE>::T T;
     typedef Record<TYPE, GROUPS, ROWS, ZEROS> R;
     constexpr int NT = R::NT, MTW = R::TILES, STEPS = R::STEPS, PIECES = R::PIECES, RUN = STEPS / GROUPS, SETS = R::CODES_AHEAD;
-    // A record is fetched in LOADS rounds of 8 KB.  Round l is put into LDS beside tile slot(l) of the stage before its
-    // own and fetched AHEAD tiles earlier: half a stage where the rounds divide by two, which
-    // needs half the registers, else a whole one.
-    constexpr int LOADS = (R::OPERANDS + 7) / 8, AHEAD = LOADS % 2 == 0 ? MTW / 2 : MTW, HELD = LOADS % 2 == 0 ? LOADS / 2 : LOADS;
+    // A record is fetched in LOADS rounds of 8 KB, an even number.  Round l is put into LDS beside tile slot(l) of the stage
+    // before its own and fetched AHEAD tiles earlier, half a stage, so that half of the rounds are in registers.
+    static_assert(R::OPERANDS % 16 == 0, "two halves of whole rounds");
+    constexpr int LOADS = R::OPERANDS / 8, AHEAD = MTW / 2, HELD = LOADS / 2;
     constexpr int SUM_LOADS = (R::SUMS + 511) / 512;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -134,8 +134,7 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
     const unsigned char* records = a.records + (size_t)band * a.stages * R::BYTES;
     auto record_of = [&](int stage) { return records + (size_t)min(stage, s1 - 1) * R::BYTES; };   // past the last: fetched again, not used
     auto slot = [](int l) { return l * MTW / LOADS; };
-    // (where the waves do not share a record out evenly, some of the last round fetch and put the same)
-    auto part = [&](int l) { return (l + 1) * 8 <= R::OPERANDS ? l * 8 + wave : min(l * 8 + wave, R::OPERANDS - 1); };
+    auto part = [&](int l) { return l * 8 + wave; };
     uintx4 next[HELD];
     typedef typename std::conditional<ZEROS, uintx4, float>::type Sum;
     Sum next_sum[SUM_LOADS];
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(512, 2) void linear_q4_band_kernel(BandArgs a)
                 if (slot(l) == mt) put(l, now ^ 1);
 #pragma unroll
             for (int l = 0; l < LOADS; ++l)
-                if (slot(l) == (mt + AHEAD) % MTW) fetch(l, AHEAD < MTW && mt < AHEAD ? from1 : from2);
+                if (slot(l) == (mt + AHEAD) % MTW) fetch(l, mt < AHEAD ? from1 : from2);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const int turn = (mt * GROUPS + g) & 1;
