@@ -341,3 +341,61 @@ def test_a_batch_taken_in_passes(shape):
     assert torch.equal(g, out)
     del room, out, g, ws, x, a
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(2100, 2300), (2300, 2100), (1030, 4111), (4111, 1030), (4000, 4100), (5000, 3333)], ids=lambda s: "x".join(map(str, s)))
+def test_orthogonalize_large_tiles(shape):
+    """Every size of tile, sliced and not, with sides that are no multiple of it, after one step, two and five.  Few large
+    singular values, so that the products weigh as much as x itself: a part left out of one of them is 2^-12 of the result.
+    C of the bar above allows for sides of some 400; the random part of longer sums grows with their root."""
+    m, n = shape
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    g = torch.randn(m, 5, device="cuda", generator=gen) @ torch.randn(5, n, device="cuda", generator=gen) + 0.3 * torch.randn(m, n, device="cuda", generator=gen)
+    for steps in (1, 2, 5):
+        print(f"orthogonalize {shape} steps={steps}", flush=True)
+        out = tl.orthogonalize(g, steps=steps)
+        x = (g if m <= n else g.t().contiguous()).double()
+        x = x / (x.norm() + 1e-7)
+        bar = float(x.norm()) * 3.4445 ** steps
+        for i in range(1, steps + 1):
+            a = x @ x.t().contiguous()
+            x = USUAL[0] * x + (USUAL[1] * a + USUAL[2] * (a @ a)) @ x
+            bar += float(x.norm()) * 3.4445 ** (steps - i)
+        far = float((out.double() - (x if m <= n else x.t())).norm())
+        assert far <= 32 * max(1.0, (max(m, n) / 400) ** 0.5) * 2.0 ** -24 * bar, (far, bar)
+
+
+def test_rows_of_very_different_size():
+    """Rows down to 1e-7 of the others: each value within 2^-39 of the norm a kept value may be off by, enlarged as the bar
+    above enlarges it, and the whole within that bar."""
+    for shape in ((60, 100), (300, 500)):
+        g = _gradient(*shape, seed=8) * torch.logspace(0, -7, shape[0])[:, None]
+        print(f"orthogonalize rows of different size {shape}", flush=True)
+        for steps in (1, 5):
+            _check(tl.orthogonalize(g.cuda(), steps=steps), g, steps)
+
+
+def test_the_optimiser_on_16_bit_layers():
+    """Steps on bf16 and fp16 matrices, some of one shape, against the formula in 64 bits: state to 32 bits, weights to one rounding."""
+    for t in (torch.bfloat16, torch.float16):
+        gen = torch.Generator().manual_seed(1)
+        shapes = [(40, 24), (40, 24), (200, 300)]
+        ws = [torch.nn.Parameter((torch.randn(s, generator=gen) * 0.1).to(t).cuda()) for s in shapes]
+        w64 = [w.detach().double().cpu() for w in ws]
+        b64 = [torch.zeros_like(w) for w in w64]
+        opt = tl.cake_muon(ws, lr=0.05, momentum=0.9, weight_decay=0.1)
+        bars = [0.0] * 3
+        for step in range(3):
+            for i, (m, n) in enumerate(shapes):
+                ws[i].grad = _gradient(m, n, 10 * step + i).to(t).cuda()
+                b64[i] = 0.9 * b64[i] + ws[i].grad.double().cpu()
+                o, bar = _reference(ws[i].grad.double().cpu() + 0.9 * b64[i], 5, USUAL, 1e-7, 3.4445)
+                scale = 0.05 * max(1.0, m / n) ** 0.5
+                w64[i] = w64[i] * (1 - 0.05 * 0.1) - scale * o
+                # the orthogonal part's bar, enlarged by what u's own rounding adds (2^-22 of its norm, L^5), and the 32-bit weight's roundings
+                bars[i] += scale * (bar + 2.0 ** -22 * 3.4445 ** 5) + 4 * 2.0 ** -24 * float(w64[i].norm())
+            opt.step()
+            for w, want, bar in zip(ws, w64, bars):
+                assert opt.state[w]["momentum"].dtype == opt.state[w]["weight"].dtype == torch.float32
+                assert float((opt.state[w]["weight"].double().cpu() - want).norm()) <= bar, step
+                assert torch.equal(w.detach(), opt.state[w]["weight"].to(t))

@@ -420,3 +420,126 @@ def test_an_input_of_huge_values(kind):
             assert float(x.abs().max()) > 1e36
             print(f"linear_q4 huge M={M} {kind} group={group} zeros={zeros}", flush=True)
             _check(tl.forward_q4(x.cuda(), q), x, v64, mass, None, K)
+
+
+def _on_device(y, x, v64, mass, bias, K, R=None):
+    """_check with the 64-bit sums on the device"""
+    x64, v, s = x.double(), v64.cuda(), mass.cuda()
+    want = x64 @ v.t().contiguous()
+    S = x64.abs() @ s.t().contiguous()
+    if bias is not None:
+        want, S = want + bias.double(), S + bias.double().abs()
+    tol = (R or 16 * (-(-K // 128)) + 48) * 2.0 ** -24 * S + 2.0 ** -40
+    if y.dtype != torch.float32:
+        tol = tol + torch.finfo(y.dtype).eps / 2 * (want.abs() + tol) + (2.0 ** -25 if y.dtype == torch.float16 else 0)
+    far = (y.double() - want).abs() - tol
+    assert y.shape == want.shape and bool((far <= 0).all()), float(far.max())
+
+
+KINDS = [(group, zeros, scale) for zeros in (False, True) for group, scale in ((32, "bf16"), (64, "f16"), (128, "f32"))]
+
+
+@pytest.mark.parametrize("shape", [(300, 16500, 200), (600, 8200, 200), (1100, 8200, 300), (2050, 4100, 300), (1030, 4111, 1500)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_prompts_in_wide_bands(shape, kind):
+    """What fills the device is taken in bands of 128 rows, or 256 for 16-bit x without zero points: last bands and strips
+    that are partly filled, blocks that end inside K, every group size, with and without zero points."""
+    M, N, K = shape
+    for i, (group, zeros, scale) in enumerate(KINDS):
+        packed, s, z, v64, mass = _weights(N, K, group, zeros, TYPES[scale], i)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+        gen = torch.Generator(device="cuda").manual_seed(i)
+        x = torch.randn(M, K, device="cuda", generator=gen).to(TYPES[kind])
+        bias = torch.randn(N, device="cuda", generator=gen).to(TYPES[kind]) if i % 2 else None
+        around = torch.full((M * N + 64,), 7.0, dtype=TYPES[kind], device="cuda")
+        y = around[:M * N].view(M, N)
+        print(f"linear_q4 M={M} N={N} K={K} {kind} group={group} zeros={zeros}", flush=True)
+        cake.linear_q4_forward(x, q, bias, y, M, timed=False)
+        _on_device(y, x, v64, mass, bias, K)
+        assert bool((around[M * N:] == 7).all())
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 6, 10, 11, 40, 600])
+def test_every_bit_of_a_32_bit_input_counts(rows):
+    """One element of 24 significant bits a row, at the ends of steps, runs and blocks: a result is s (code - z) x with
+    no more than 12 roundings in a row (three pieces' sums, zero points and scales, and their joining); without the last
+    8 bits of x it would be off by up to 256 times 2^-24."""
+    K, N = (200, 8200) if rows == 600 else (300, 75)
+    columns = [c for c in (0, 7, 8, 31, 32, 63, 64, 95, 96, 127, 128, 191, 199, 255, 256, 287, 288, 299) if c < K]
+    for i, (group, zeros, scale) in enumerate(KINDS):
+        packed, s, z, v64, mass = _weights(N, K, group, zeros, TYPES[scale], 20 + i)
+        q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+        for turn in range(len(columns) if rows < 3 else 3):
+            x = torch.zeros(rows, K)
+            gen = torch.Generator().manual_seed(turn)
+            bits = torch.randint(1 << 22, 1 << 23, (rows,), generator=gen) * 2 + 1      # 24 bits, the first and the last set
+            for m in range(rows):
+                x[m, columns[(turn + m) % len(columns)]] = float(bits[m]) * 2.0 ** -22 * (-1) ** m
+            print(f"linear_q4 24 bits M={rows} group={group} zeros={zeros}", flush=True)
+            _on_device(tl.forward_q4(x.cuda(), q), x.cuda(), v64, mass, None, K, R=12)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_inputs_with_outliers_and_an_offset(kind):
+    """Columns a thousand times the others, some of them where every code is the zero point, and rows that do not sum to
+    nothing: within the bar, whose S counts code and zero point apart."""
+    N, K = 130, 700
+    for group, zeros in ((32, True), (64, False), (128, True), (128, False)):
+        packed, s, z, _, _ = _weights(N, K, group, zeros, torch.float32, 6)
+        packed[:, 5::16] = 0x88
+        k = torch.arange(K)
+        code = ((packed[:, k // 2].int() >> (4 * (k % 2)).int()) & 15).double()
+        if zeros:
+            z = z.round()
+            z[::2] = 8
+        z64 = z.double()[:, k // group] if zeros else torch.full((N, K), 8.0, dtype=torch.float64)
+        s64 = s.double()[:, k // group]
+        q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda() if zeros else None, K, group)
+        for M in (1, 4, 9, 20, 33, 200):
+            x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)) + 3
+            x[:, 10::32] *= 1000
+            x = x.to(TYPES[kind]).cuda()
+            print(f"linear_q4 outliers M={M} {kind} group={group} zeros={zeros}", flush=True)
+            _on_device(tl.forward_q4(x, q), x, (code - z64) * s64, s64 * (code + z64), None, K)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradients_of_larger_layers(kind):
+    """A layer of a thousand columns, rows from none to some hundreds, either gradient alone."""
+    N, K, t = 1001, 1300, TYPES[kind]
+    packed, s, z, v64, _ = _weights(N, K, 32, True, torch.bfloat16, 9)
+    q = tl.pack_q4(packed.cuda(), s.cuda(), z.cuda(), K, 32)
+    v = v64.cuda()
+    for M in (0, 1, 17, 300):
+        gen = torch.Generator(device="cuda").manual_seed(M)
+        x0, gy = torch.randn(M, K, device="cuda", generator=gen).to(t), torch.randn(M, N, device="cuda", generator=gen).to(t)
+        b0 = torch.randn(N, device="cuda", generator=gen).to(t)
+        for need_x, need_b in ((True, True), (True, False), (False, True)):
+            x, b = x0.clone().requires_grad_(need_x), b0.clone().requires_grad_(need_b)
+            print(f"backward M={M} {kind} {need_x} {need_b}", flush=True)
+            tl.forward_q4(x, q, b).backward(gy)
+            g64 = gy.double()
+            if need_x:
+                want = g64 @ v
+                # N products and the rounding of each weight to 32 bits, then the type (and fp16's last subnormal step)
+                tol = (N + 8) * 2.0 ** -24 * (g64.abs() @ v.abs()) + (torch.finfo(t).eps / 2 * want.abs() * 1.01 + 2.0 ** -25 if t != torch.float32 else 0)
+                assert x.grad.dtype == t and x.grad.shape == x.shape and bool(((x.grad.double() - want).abs() <= tol).all())
+            if need_b:
+                want = g64.sum(0)
+                tol = M * 2.0 ** -24 * g64.abs().sum(0) + (torch.finfo(t).eps / 2 * want.abs() * 1.01 + 2.0 ** -25 if t != torch.float32 else 0)
+                assert b.grad.dtype == t and bool(((b.grad.double() - want).abs() <= tol).all())
+
+
+def test_a_workspace_in_host_memory_is_refused():
+    N, K, M = 64, 128, 50
+    q = tl.quantize_q4(torch.ones(N, K, device="cuda"), 128)
+    x, y = torch.ones(M, K, device="cuda"), torch.full((M, N), 7.0, device="cuda")
+    lib = cake.load()
+    need = lib.cake_hip_linear_q4_workspace(M, N, K, _lib.F32)
+    host = np.zeros(need + 16, np.uint8)
+    at = host.ctypes.data + (-host.ctypes.data % 16)
+    st = lib.cake_hip_linear_q4_forward(x.data_ptr(), q.data.data_ptr(), None, y.data_ptr(), _lib.F32, M, N, K, 128, _lib.BF16, 0, at, None, None)
+    assert need > 0 and st == _lib.ERR_ARG and b"workspace" in lib.cake_hip_last_error()
+    torch.cuda.synchronize()
+    assert bool((y == 7).all()) and not host.any()
