@@ -565,6 +565,9 @@ class Q4Weight:
     def __setattr__(self, name, value):
         raise AttributeError(f"packed weights are made for one {name}; q4_of wraps other bytes")
 
+    def __repr__(self):   # of what is in it and not of where it lies: a trace compares it with the next one's
+        return f"Q4Weight(N={self.N}, K={self.K}, group={self.group}, scale_type={self.scale_type}, with_zeros={self.with_zeros})"
+
     def __reduce__(self):
         return Q4Weight, (self.data, self.N, self.K, self.group, self.scale_type, self.with_zeros)
 

@@ -116,20 +116,6 @@ def _watched():
     return _is_tracing() or forward_ad._current_level >= 0
 
 
-class _recorded_function(torch.autograd.Function):
-    """compute(tensor) as one operation of a trace; it has no gradient."""
-
-    @staticmethod
-    def forward(ctx, tensor, compute):
-        out = compute(tensor.detach())
-        ctx.mark_non_differentiable(out)
-        return out
-
-    @staticmethod
-    def backward(ctx, grad_output):
-        return None, None
-
-
 def _not_in_a_trace(what):
     if _is_tracing():
         raise RuntimeError(f"{what}: a trace cannot record what packs weights; pack them before it and trace the layer")
@@ -163,12 +149,22 @@ def quantize_q4(weight, group=128, zeros=False, scale_dtype=torch.bfloat16):
 
 def dequantize_q4(q, dtype=torch.float32):
     """The values that packed weights stand for, as a tensor [N][K]."""
-    def values(packed):
-        w = torch.empty((q.N, q.K), dtype=dtype, device=packed.device)
-        api.q4_dequantize(q if packed is q.data else api.Q4Weight(packed, q.N, q.K, q.group, q.scale_type, q.with_zeros), w)
-        return w
+    call = _dequantize_q4_function.apply if _is_tracing() else _dequantize_q4
+    return call(q.data, q.N, q.K, q.group, q.scale_type, q.with_zeros, dtype)
 
-    return _recorded_function.apply(q.data, values) if _is_tracing() else values(q.data)
+
+def _dequantize_q4(packed, N, K, group, scale_type, with_zeros, dtype):
+    w = torch.empty((N, K), dtype=dtype, device=packed.device)
+    api.q4_dequantize(api.Q4Weight(packed, N, K, group, scale_type, with_zeros), w)
+    return w
+
+
+class _dequantize_q4_function(torch.autograd.Function):
+    """As one operation of a trace, on plain numbers, which are the same in every trace; packed weights are constants."""
+
+    @staticmethod
+    def forward(ctx, packed, *args):
+        return _dequantize_q4(packed, *args)
 
 
 def _forward_q4(input, q, bias):
@@ -288,9 +284,16 @@ def orthogonalize(grad, steps=5, coefficients=api.NEWTON_SCHULZ, eps=1e-7):
     matrices have their singular values moved close to 1.  Not differentiable."""
     if grad.dim() < 2:
         raise ValueError(f"orthogonalize: {tuple(grad.shape)} is no matrix")
-    if _is_tracing():
-        return _recorded_function.apply(grad, lambda g: _orthogonalize(g, steps, coefficients, eps))
-    return _orthogonalize(grad.detach(), steps, coefficients, eps)
+    call = _orthogonalize_function.apply if _is_tracing() else _orthogonalize
+    return call(grad.detach(), steps, coefficients, eps)
+
+
+class _orthogonalize_function(torch.autograd.Function):
+    """As one operation of a trace."""
+
+    @staticmethod
+    def forward(ctx, grad, steps, coefficients, eps):
+        return _orthogonalize(grad, steps, coefficients, eps)
 
 
 def _orthogonalize(grad, steps, coefficients, eps):

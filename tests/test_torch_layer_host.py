@@ -308,3 +308,14 @@ def test_packed_weights_are_copied_and_stored_whole():
     for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
         assert torch.equal(other.data, q.data) and (other.N, other.K, other.group, other.scale_type, other.with_zeros) == (N, K, 32, _lib.F32, False)
     assert copy.deepcopy(q).data.data_ptr() != q.data.data_ptr()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_trace_compares_equal_with_the_next_one(stand_ins, grad):
+    """torch.jit.trace's own check, which records everything twice and refuses what differs."""
+    layer, q = _layer(3, True), cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    with torch.set_grad_enabled(grad):
+        for call in (layer, lambda v: tl.forward_q4(v, layer.weight_q4), lambda v: tl.orthogonalize(v), lambda v: v @ tl.dequantize_q4(q).t()):
+            traced = torch.jit.trace(call, (torch.randn(4, K),))
+            x = torch.randn(6, K)
+            assert torch.equal(traced(x), call(x))
