@@ -543,3 +543,19 @@ def test_a_workspace_in_host_memory_is_refused():
     assert need > 0 and st == _lib.ERR_ARG and b"workspace" in lib.cake_hip_last_error()
     torch.cuda.synchronize()
     assert bool((y == 7).all()) and not host.any()
+
+
+@pytest.mark.parametrize("N", [50, 8200])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_rows_under_every_kind_of_weights(kind, N):
+    """Every group size with every type of scales, for the numbers of rows that fill a result register, one tile and two."""
+    K = 300
+    for group in (32, 64, 128):
+        for i, scale in enumerate(TYPES):
+            zeros = (group // 32 + i) % 2 == 0
+            packed, s, z, v64, mass = _weights(N, K, group, zeros, TYPES[scale], 40 + i)
+            q = tl.pack_q4(packed.cuda(), s.cuda(), None if z is None else z.cuda(), K, group)
+            for M in (1, 5, 9, 18):
+                x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(TYPES[kind]).cuda()
+                print(f"linear_q4 M={M} N={N} {kind} group={group} scales={scale} zeros={zeros}", flush=True)
+                _on_device(tl.forward_q4(x, q), x, v64, mass, None, K)
