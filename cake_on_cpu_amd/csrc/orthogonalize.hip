@@ -8,7 +8,8 @@
 // iteration's values are bounded by its coefficients, so e is known beforehand).  A product is then
 // hi hi + hi lo + lo hi -- three matrix instructions where the fp32 ones, at a sixteenth of the rate,
 // would take the time of sixteen -- summed in 32 bits; lo lo is at most 2^-22 of the product, of
-// either sign.  The floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39.
+// either sign.  The floor under lo is 2^-25 of the scaled value: with e = 14, 2^-39, which rows far smaller than the others
+// come to feel (at 1e-5 of them 2e-6 of themselves, at 1e-7 2e-4, after 5 steps; the whole stays at 1.3e-6, plain fp32 at 1.7e-6).
 // b is kept without c0 I, and in the first step and while four or more follow x is carried in fp32 beside its
 // pairs: early steps are little more than x = c0 x, and what is lost of a small singular value there
 // is enlarged by every later step (final error on a 1024 x 1024 gradient: 4.2e-7 carried to the end,

@@ -223,8 +223,8 @@ class cake_linear_q4_function(torch.autograd.Function):
 
 def forward_q4(input, q, bias=None):
     """output[M][N] = input[M][K] . v[N][K]^T (+ bias) with v in 4 bits (pack_q4, quantize_q4).  input is float32,
-    float16 or bfloat16, bias and output likewise; sums are fp32.  Differentiable in input and bias (reverse
-    mode; a tangent of forward mode is refused)."""
+    float16 or bfloat16, bias and output likewise; sums are fp32, of codes and of zero points apart (include/cake_hip.h
+    says what that leaves of outliers).  Differentiable in input and bias (reverse mode; a tangent of forward mode is refused)."""
     if (torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad))) or _watched():
         return cake_linear_q4_function.apply(input, q, bias, q.data)
     return _forward_q4(input, q, bias)
@@ -281,7 +281,8 @@ class cake_linear_q4(nn.Module):
 
 def orthogonalize(grad, steps=5, coefficients=api.NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz iterations on the last two dimensions (leading ones are a batch): a tensor like `grad` whose
-    matrices have their singular values moved close to 1.  Not differentiable."""
+    matrices have their singular values moved close to 1.  Not differentiable.  Rows and columns down to 1e-3 of the others
+    are as exact as these, smaller ones less (include/cake_hip.h)."""
     if grad.dim() < 2:
         raise ValueError(f"orthogonalize: {tuple(grad.shape)} is no matrix")
     call = _orthogonalize_function.apply if _is_tracing() else _orthogonalize

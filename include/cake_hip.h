@@ -448,8 +448,12 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
 
 /* y[M][N] = x[M][K] . v[N][K]^T (+ bias[N] on every row when bias != NULL); x, bias and y are of `type`.
  * The weights are not rounded on the way: products of x and whole codes are summed in fp32, scales and
- * zero points are applied to a run's sums in fp32, and y is rounded once.  The order of the sums depends
- * on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
+ * zero points are applied to a run's sums in fp32, and y is rounded once.  The sums of codes and of zero points
+ * cancel, so an error counts in last places of sum s (c + |z|) |x|, not of sum |v| |x|: a large x at a code that equals its zero
+ * point adds nothing to y and still leaves some last places of 8 s |x| (fp32 x with one column of 128 a thousand times
+ * the others, every code there the zero point: y off by 3e-5 of itself, by 5e-7 with fp32 products of v; with x
+ * of one size 1e-7 to 3e-7).  Sums do not overflow where the values do not.  An fp32 x counts with its 24 bits down to 2^-110, with
+ * fewer below.  The order of the sums depends on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
  * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 24 rows of
  * x, 10 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
  * streams, two captured graphs) need workspaces of their own. */
@@ -469,7 +473,8 @@ int cake_hip_linear_q4_forward(const void* x, const void* q, const void* bias, v
  * count as they are, the result is rounded once).  Singular values start in 0..1; coefficients whose
  * polynomial takes them beyond 1000 within `steps` are refused (CAKE_HIP_ERR_ARG).  x is kept to
  * 2^-23 of each value and no finer than 2^-39 (for the coefficients above), so a g whose
- * norm lies below about 1e-4 eps loses relative accuracy.  A matrix of zeros gives zeros; one that holds a NaN
+ * norm lies below about 1e-4 eps loses relative accuracy, and so do rows or columns far smaller than the others: at 1e-3 of
+ * them they come out as exact as the rest (3e-7 of themselves after 5 steps), at 1e-5 to 2e-6, at 1e-7 to 2e-4.  A matrix of zeros gives zeros; one that holds a NaN
  * or an infinity gives NaN and leaves the rest of the batch alone.
  * Matrices of more than 2^26 values together are taken some at a time, so the workspace stays within some 1.5 GB or what one
  * matrix needs (16 to 24 bytes a value).
