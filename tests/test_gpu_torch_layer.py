@@ -66,3 +66,29 @@ def test_a_traced_layer_computes_on_the_device(rows):
             for _ in range(3):
                 x, g = torch.randn(rows, 300, device="cuda"), torch.randn(40, 60, device="cuda")
                 assert torch.equal(traced(x), layer(x)) and torch.equal(update(g), tl.orthogonalize(g))
+
+
+@pytest.mark.parametrize("rows", [1, 7, 100])
+def test_gradients_through_a_traced_layer(rows):
+    layer = tl.cake_linear_q4.of(tl.cake_linear(300, 130).cuda(), group=64, zeros=True)
+    traced = torch.jit.trace(layer, (torch.randn(rows, 300, device="cuda"),))
+    for _ in range(3):
+        x, gy = torch.randn(rows, 300, device="cuda", requires_grad=True), torch.randn(rows, 130, device="cuda")
+        want = torch.autograd.grad(layer(x), (x, layer.bias), gy)
+        got = torch.autograd.grad(traced(x), (x, layer.bias), gy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_compiled_model_calls_the_layer(grad):
+    """torch.compile leaves the calls as they are and compiles around them."""
+    layer = tl.cake_linear_q4.of(tl.cake_linear(300, 130).cuda(), group=64)
+
+    def model(x):
+        return torch.relu(layer(x * 2)) + 1
+
+    compiled = torch.compile(model, backend="eager")
+    with torch.set_grad_enabled(grad):
+        for rows in (1, 7, 7, 100):
+            x = torch.randn(rows, 300, device="cuda")
+            assert torch.equal(compiled(x), model(x))
