@@ -11,8 +11,8 @@
 // more.  Inside a dword, byte b has element b in its low and element b + 4 in its high nibble:
 // a mask (and a shift) leaves four codes as four bytes, and a byte 0..15 read as an 8-bit float
 // (4 exponent and 3 mantissa bits, bias 7) is code * 2^-9 exactly -- 0..7 as subnormals, 8..15 with
-// the exponent's last bit -- so the hardware's conversion of two such bytes with the scale 2^9 gives
-// two codes as 16-bit floats: 7 vector instructions for 8 weights.
+// the exponent's last bit -- so the hardware's conversion of two such bytes with a scale of 2^9 gives
+// two codes as 16-bit floats (or in units of 2^-12, with 2^-3): 7 vector instructions for 8 weights.
 // Behind the codes (at the next multiple of 256 bytes) lie the scales as [tile][block][row][128 / group]
 // in their own type, then the zero points likewise.  Rows past N and columns past K hold code 0
 // under scale 0.
