@@ -571,6 +571,9 @@ class Q4Weight:
     def __reduce__(self):
         return Q4Weight, (self.data, self.N, self.K, self.group, self.scale_type, self.with_zeros)
 
+    def __setstate__(self, state):   # what was stored attribute by attribute
+        self.__init__(**state[1])
+
 
 def _q4_bytes(N, K, group, scale_type, zeros) -> int:
     n = load().cake_hip_q4_size(N, K, group, scale_type, bool(zeros))

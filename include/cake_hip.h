@@ -452,8 +452,8 @@ int cake_hip_q4_dequantize(const void* q, void* w, int w_type, int N, int K, int
  * cancel, so an error counts in last places of sum s (c + |z|) |x|, not of sum |v| |x|: a large x at a code that equals its zero
  * point adds nothing to y and still leaves some last places of 8 s |x| (fp32 x with one column of 128 a thousand times
  * the others, every code there the zero point: y off by 3e-5 of itself, by 5e-7 with fp32 products of v; with x
- * of one size 1e-7 to 3e-7).  Sums do not overflow where the values do not.  An fp32 x counts with its 24 bits down to 2^-110, with
- * fewer below.  The order of the sums depends on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
+ * of one size 1e-7 to 3e-7).  With zero points up to 16 no sum overflows as long as sum |v| |x| does not.  An fp32 x
+ * counts with its 24 bits down to 2^-110 and a y down to 2^-113, with fewer below.  The order of the sums depends on the sizes, types and groups alone.  M stays below 2^29.  An infinity in x may come out as NaN in that row of y.  K == 0
  * gives y = bias or 0.  workspace: device memory of cake_hip_linear_q4_workspace bytes (0 for up to 24 rows of
  * x, 10 of fp32), 16-byte aligned, or NULL for a buffer of the context's own; calls that overlap (two
  * streams, two captured graphs) need workspaces of their own. */

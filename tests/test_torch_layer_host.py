@@ -319,3 +319,11 @@ def test_a_trace_compares_equal_with_the_next_one(stand_ins, grad):
             traced = torch.jit.trace(call, (torch.randn(4, K),))
             x = torch.randn(6, K)
             assert torch.equal(traced(x), call(x))
+
+
+def test_packed_weights_stored_attribute_by_attribute_load():
+    """As pickle stores an object with slots by itself, which is how they were stored before their numbers were fixed."""
+    q = cake.q4_of(_packed(3), N, K, 32, "float32", False)
+    other = cake.Q4Weight.__new__(cake.Q4Weight)
+    other.__setstate__((None, {name: getattr(q, name) for name in ("data", "N", "K", "group", "scale_type", "with_zeros")}))
+    assert other.data is q.data and other.bytes == q.bytes and repr(other) == repr(q)
