@@ -4,13 +4,14 @@
 // Codes are whole numbers 0..15, exact in 16-bit floats, so the products go to the matrix pipe as
 // x . code and the group's scale and zero point are applied to the 32-bit sums behind it:
 //   y[m][n] = sum over groups g of s[n][g] * (sum_k x[m][k] code[n][k] - z[n][g] * sum_k x[m][k]).
-// No weight is rounded.  (Codes less their zero point would keep the two sums from cancelling, but bf16 pairs have no addition:
-// through fp32 it is 20 vector instructions for 8 codes in place of 7.)  The sums are larger than what they stand for, up to 15 x 128 of the largest x before the
-// scale is applied, so where x reaches as far as fp32 does, codes and column sums count in units of 2^-12
-// (exact, by the unpacking's own scale) and the result is multiplied by 2^12 at its end: no sum overflows where the
-// values do not.  x is exact as well: 16-bit types go in as they are, a 32-bit x as three
-// bf16 pieces (its leading, middle and last 8 significant bits, cut, not rounded, so that no piece
-// overflows) that take three rows of the product and are added up at the end.
+// No weight is rounded.  (Codes less their zero point would keep the two sums from cancelling, but bf16 pairs
+// have no addition: through fp32 it is 20 vector instructions for 8 codes in place of 7.)  The sums are larger
+// than what they stand for, up to 15 x 128 of the largest x before the scale is applied, so where x reaches as
+// far as fp32 does, codes and column sums count in units of 2^-12 (exact, by the unpacking's own scale) and the
+// result is multiplied by 2^12 at its end: no sum overflows where the values do not.  x is exact as well:
+// 16-bit types go in as they are, a 32-bit x as three bf16 pieces (its leading, middle and last 8 significant
+// bits, cut, not rounded, so that no piece overflows) that take three rows of the product and are added up at
+// the end.
 #pragma once
 
 #include "low_bits.hpp"

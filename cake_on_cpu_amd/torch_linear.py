@@ -318,9 +318,9 @@ class cake_muon(torch.optim.Optimizer):
     other vectors belong to another optimiser):
         b = momentum * b + grad,  u = grad + momentum * b  (b without nesterov)
         w = w - lr * weight_decay * w - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
-    Matrices of one shape are orthogonalised together, up to 2^26 values in a call.  The state is kept in fp32 whatever the parameters' type (float32,
-    float16, bfloat16): the momentum, and of a 16-bit w an fp32 copy that the formula runs on and w is rounded from, so that
-    updates below a step of w's type add up.  A w that was set from elsewhere counts as it was set."""
+    Matrices of one shape are orthogonalised together, up to 2^26 values in a call.  The state is kept in fp32 whatever the
+    parameters' type (float32, float16, bfloat16): the momentum, and of a 16-bit w an fp32 copy that the formula runs on and
+    w is rounded from, so that updates below a step of w's type add up.  A w that was set from elsewhere counts as it was set."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=api.NEWTON_SCHULZ,
                  eps=1e-7):
